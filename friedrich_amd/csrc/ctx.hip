@@ -425,13 +425,10 @@ int fr_ctx_create(fr_ctx** out, int device)
     }
     ctx->own_stream = true;
     ctx->ls = ctx->stream;
-    int lo = 0, hi = 0;
-    (void)hipDeviceGetStreamPriorityRange(&lo, &hi);  // hi = numerically lowest = highest priority
-    // Only the panel / chain stream is high-priority.  The bulk stream of the chain-first schedule carries what is explicitly
-    // NOT on the critical path (slice solves, copies, the large collectives): default priority, so that it neither competes
-    // with the chain nor pre-empts the main stream's updates (round 1 measured a busy high-priority queue throttling the
-    // dispatch of the others: +16 % on trailing updates).
-    if (hipStreamCreateWithPriority(&ctx->stream2, hipStreamNonBlocking, hi) != hipSuccess ||
+    // Every stream has the default priority: work on queues of different priorities has hung on this hardware for good, and a busy
+    // high-priority queue throttled the dispatch of the others (+16 % on trailing updates).  The panel chain gets its room from
+    // the reservation of CUs instead (gemm_f64.hip), not from the queue.
+    if (hipStreamCreateWithFlags(&ctx->stream2, hipStreamNonBlocking) != hipSuccess ||
         hipStreamCreateWithFlags(&ctx->stream3, hipStreamNonBlocking) != hipSuccess ||
         hipEventCreateWithFlags(&ctx->ev_bulk, hipEventDisableTiming) != hipSuccess ||
         hipEventCreateWithFlags(&ctx->ev_cols, hipEventDisableTiming) != hipSuccess ||

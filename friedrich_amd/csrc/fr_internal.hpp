@@ -58,7 +58,7 @@ struct fr_ctx {
     hipStream_t stream = nullptr;   // main stream (memcpys, host synchronisation)
     bool own_stream = true;
     hipStream_t ls = nullptr;       // stream the kernel launchers enqueue on (== stream except inside look-ahead)
-    hipStream_t stream2 = nullptr;  // high-priority panel stream of the look-ahead Cholesky
+    hipStream_t stream2 = nullptr;  // panel stream of the look-ahead Cholesky (default priority: ctx.hip)
     hipStream_t stream3 = nullptr;  // sharded factorisation: the bulk rows of a panel (solves + all-gather) off the diagonal chain
     hipEvent_t ev_panel = nullptr, ev_la = nullptr, ev_cols = nullptr, ev_bulk = nullptr;
     int64_t cols_final_at = -1;     // factor_panel records ev_cols when the columns up to this one are final (look-ahead pipeline)

@@ -123,9 +123,8 @@ int main(int argc, char** argv)
         (void)hipMemset(NC, 0, NM * NM * 8);
     }
     hipStream_t hs;
-    int lo_p, hi_p;
-    (void)hipDeviceGetStreamPriorityRange(&lo_p, &hi_p);
-    (void)hipStreamCreateWithPriority(&hs, hipStreamNonBlocking, hi_p);
+    
+    (void)hipStreamCreateWithFlags(&hs, hipStreamNonBlocking);
     double* out;
     long long* ts;
     (void)hipMalloc(&out, 8 * 64);

@@ -4,7 +4,7 @@
 //   hog:   workgroups with the trailing update's footprint (240 VGPRs, 73 KB LDS: two per CU), exit at once on the reserved
 //          XCDs, spin `hog_us` elsewhere; enough of them for `rounds` rounds                                  (main stream)
 //   panel: G workgroups with the 32-row tile's footprint (176 VGPRs, 49 KB LDS), work 10 us on the reserved XCDs, exit at once
-//          elsewhere                                                                                          (priority stream)
+//          elsewhere                                                                                          (a second stream)
 // Device-side stamps (s_memrealtime, 100 MHz): first hog start, first / last panel workgroup start, last panel end.
 #include <hip/hip_runtime.h>
 #include <cstdio>
@@ -65,10 +65,8 @@ __global__ void where(unsigned* out)
 int main()
 {
     hipStream_t sm, sp;
-    int lo, hi;
-    CK(hipDeviceGetStreamPriorityRange(&lo, &hi));
     CK(hipStreamCreateWithFlags(&sm, hipStreamNonBlocking));
-    CK(hipStreamCreateWithPriority(&sp, hipStreamNonBlocking, hi));
+    CK(hipStreamCreateWithFlags(&sp, hipStreamNonBlocking));
     CK(hipFuncSetAttribute((const void*)hog, hipFuncAttributeMaxDynamicSharedMemorySize, 73736));
     CK(hipFuncSetAttribute((const void*)panel, hipFuncAttributeMaxDynamicSharedMemorySize, 49160));
     unsigned* d;
@@ -80,7 +78,7 @@ int main()
     CK(hipStreamSynchronize(sp));
     unsigned x0 = 0;
     CK(hipMemcpy(&x0, d, 4, hipMemcpyDeviceToHost));
-    printf("priority stream: single-workgroup launches run on XCD %u\n", x0);
+    printf("second stream: single-workgroup launches run on XCD %u\n", x0);
     for (unsigned nres : {2u}) {
         const int need = 156, grid = need * 8 / (int)nres;
         for (int rounds : {1, 3}) {

@@ -10,11 +10,16 @@ mkdir -p "$(dirname "$OUT")"
 TMP=$(mktemp -d)
 {
   echo "# kernel | VGPRs | AGPRs | scratch B/lane | LDS B (static) | occupancy waves/SIMD | SGPRs | VGPRs spilled | SGPRs spilled"
-  echo "# hipcc $(/opt/rocm/bin/hipcc --version | grep -m1 'HIP version'); flags: --offload-arch=gfx950 -O3 (friedrich_amd/build.py); generated by scripts/kernel_resources.sh"
+  echo "# hipcc $(/opt/rocm/bin/hipcc --version | grep -m1 'HIP version'); flags: --offload-arch=gfx950 -O3 -packed-fp32-ops (friedrich_amd/build.py); generated by scripts/kernel_resources.sh"
+  for f in friedrich_amd/csrc/*.hip; do  # the compilations run side by side, the records are read in the order of the files
+    /opt/rocm/bin/hipcc -x hip --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fno-gpu-rdc -Xclang -target-feature -Xclang -packed-fp32-ops -Iinclude -Ifriedrich_amd/csrc -I/opt/rocm/include \
+      -Rpass-analysis=kernel-resource-usage -c "$f" -o "$TMP/$(basename "$f").o" 2> "$TMP/$(basename "$f").txt" && touch "$TMP/$(basename "$f").ok" &
+  done
+  wait
   for f in friedrich_amd/csrc/*.hip; do
-    /opt/rocm/bin/hipcc -x hip --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fno-gpu-rdc -Iinclude -Ifriedrich_amd/csrc -I/opt/rocm/include \
-      -Rpass-analysis=kernel-resource-usage -c "$f" -o "$TMP/x.o" 2> "$TMP/r.txt" || { cat "$TMP/r.txt"; exit 1; }
-    python3 - "$TMP/r.txt" "$(basename "$f")" <<'PY'
+    R="$TMP/$(basename "$f").txt"
+    [ -e "$TMP/$(basename "$f").ok" ] || { cat "$R" >&2; exit 1; }
+    python3 - "$R" "$(basename "$f")" <<'PY'
 import re, sys
 txt = open(sys.argv[1]).read()
 cur = None

@@ -14,7 +14,7 @@ CLANGXX = os.environ.get("FR_CLANGXX", "/opt/rocm/lib/llvm/bin/clang++")
 def build(force=False):
     if not force and os.path.exists(LIB) and os.path.getmtime(LIB) >= os.path.getmtime(SRC):
         return LIB
-    for cmd in ([HIPCC, "-x", "hip", "--offload-arch=gfx950", "-O2", "-std=c++17", "-fPIC", "-fno-gpu-rdc", "-I/opt/rocm/include", "-c", SRC, "-o", OBJ],
+    for cmd in ([HIPCC, "-x", "hip", "--offload-arch=gfx950", "-O2", "-std=c++17", "-fPIC", "-fno-gpu-rdc", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I/opt/rocm/include", "-c", SRC, "-o", OBJ],
                 [CLANGXX, "-shared", "-fPIC", "-o", LIB, OBJ, "-lpthread"]):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
