@@ -28,6 +28,11 @@ STATUS_NAMES = {
 FR_PROF_GRAM, FR_PROF_POTF2, FR_PROF_GEMM_PANEL, FR_PROF_SYRK, FR_PROF_GEMM_SOLVE, FR_PROF_REDUCE, FR_PROF_COMM, FR_PROF_SYRK_CHAIN = range(8)
 PROF_NAMES = ["gram", "potf2", "gemm_panel", "syrk", "gemm_solve", "reduce", "comm", "syrk_chain"]
 
+FR_LAYOUT_COLMAJOR, FR_LAYOUT_ROWMAJOR = 0, 1
+FR_F64, FR_F32, FR_BF16, FR_F16 = range(4)
+GATE_FORMS = {"value": 0, "log": 1, "stationary": 2}
+SCORES = {"softmax": 0, "sigmoid": 1}
+
 FR_KPROG_MAX_OPS = 15
 FR_COMM_ID_BYTES = 128
 
@@ -112,6 +117,14 @@ SIGNATURES = {
     "fr_panel_rows_solve": (_int, [_vp, _dp, _i64, _i64, _dp, _i64, _i64, _dp]),
     "fr_mean_pairwise_distance": (_int, [_vp, _dp, _i64, _i64, _i64, _pdbl]),
     "fr_grad_terms": (_int, [_vp, _kp, _dp, _dbl, _int, _pdbl, _pdbl]),
+    "fr_recurrence": (_int, [_vp, _int, _int, _int, _i64, _i64, _dp, _i64, _i64, _dp, _i64, _dp, _i64, _dp, _i64, _dp, _i64, _dp, _i64]),
+    "fr_recurrence_backward": (_int, [_vp, _int, _int, _int, _i64, _i64, _dp, _i64, _i64, _dp, _i64, _dp, _i64, _dp, _i64, _dp, _i64, _dp, _i64, _dp, _i64, _dp,
+                                      _i64, _dp, _i64, _dp, _i64]),
+    "fr_markov_product": (_int, [_vp, _kp, _dp, _i64, _dp, _i64, _i64, _dbl, _dp, _i64]),
+    "fr_route": (_int, [_vp, _int, _int, _int, _i64, _i64, _dp, _i64, _dp, _i64, _i64, _i64, _int, _dbl, _dp, _i64, _dp, _i64, _dp]),
+    "fr_route_backward": (_int, [_vp, _int, _int, _int, _i64, _i64, _dp, _i64, _dp, _i64, _i64, _int, _dbl, _dp, _i64, _dp, _i64]),
+    "fr_experts_predict": (_int, [_vp, _kp, _dp, _i64, _i64, _i64, _dp, _dp, _i64, _dp, _i64, _i64, _dp, _i64, _dp, _i64, _i64, _dp, _dp, _dp, _i64]),
+    "fr_experts_backward": (_int, [_vp, _kp, _dp, _i64, _i64, _i64, _dp, _i64, _dp, _i64, _i64, _dp, _i64, _dp, _i64, _i64, _dp, _i64, _dp, _dp, _i64, _dp]),
 }
 
 _lib = None

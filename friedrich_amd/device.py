@@ -104,6 +104,134 @@ def _vecptr(v):
     return a.ctypes.data, a.shape[0], a
 
 
+# ---- operands of the operators over 64-, 32- and 16-bit data ------------------------------------------------------------------------
+_DTYPES = {np.dtype(np.float64): C.FR_F64, np.dtype(np.float32): C.FR_F32, np.dtype(np.float16): C.FR_F16}
+_INTS = {np.dtype(np.int32): 4, np.dtype(np.int64): 8}
+
+
+def _code(t, table=_DTYPES):
+    """the ABI's number of an element type"""
+    code = table.get(t.dtype)
+    if code is None and _is_torch(t):
+        import torch
+
+        _DTYPES.update({torch.float64: C.FR_F64, torch.float32: C.FR_F32, torch.bfloat16: C.FR_BF16, torch.float16: C.FR_F16})
+        _INTS.update({torch.int32: 4, torch.int64: 8})
+        code = table.get(t.dtype)
+    if code is None:
+        raise ValueError(f"element type {t.dtype} is not supported here")
+    return code
+
+
+def _strides(t):
+    return t.stride() if _is_torch(t) else tuple(v // t.itemsize for v in t.strides)
+
+
+def _address(t):
+    return t.data_ptr() if _is_torch(t) else t.ctypes.data
+
+
+def _layout(*matrices):
+    """the layout of a call: that of its first matrix which has only one (a single row or column can have either)"""
+    for t in matrices:
+        if t is None:
+            continue
+        if len(t.shape) != 2:
+            raise ValueError("a matrix is needed")
+        rows, cols = t.shape
+        r, c = _strides(t)
+        col = rows <= 1 or r == 1 and (cols <= 1 or c >= rows)
+        row = cols <= 1 or c == 1 and (rows <= 1 or r >= cols)
+        if col and row:
+            continue
+        if col or row:
+            return C.FR_LAYOUT_COLMAJOR if col else C.FR_LAYOUT_ROWMAJOR
+        raise ValueError("matrices have to be contiguous along their rows or their columns")
+    return C.FR_LAYOUT_COLMAJOR
+
+
+def _lead(t, layout, shape, name):
+    """(address, leading dimension) of a matrix in the call's layout"""
+    if t is None:
+        return None, 0
+    if tuple(t.shape) != shape:
+        raise FriedrichError(C.FR_SHAPE, f"{name}: {tuple(t.shape)} where {shape} is needed")
+    rows, cols = shape
+    r, c = _strides(t)
+    if layout == C.FR_LAYOUT_COLMAJOR:
+        r, c, rows, cols = c, r, cols, rows
+    # r: from one line to the next, c: along a line
+    if (cols > 1 and c != 1) or (rows > 1 and r < cols):
+        raise ValueError(f"{name}: not in the layout of the call's other matrices")
+    return _address(t), r if rows > 1 else cols
+
+
+def _like(t, shape, layout, dtype=None):
+    """an uninitialised matrix next to t, in a layout"""
+    turn = layout == C.FR_LAYOUT_COLMAJOR
+    if _is_torch(t):
+        import torch
+
+        m = torch.empty(shape[::-1] if turn else shape, dtype=dtype or t.dtype, device=t.device)
+        return m.t() if turn else m
+    return np.empty(shape, dtype=dtype or t.dtype, order="F" if turn else "C")
+
+
+def _wide(t):
+    """the type of sums, states and weights over t"""
+    if _is_torch(t):
+        import torch
+
+        return torch.float64 if t.dtype == torch.float64 else torch.float32
+    return np.dtype(np.float64 if t.dtype == np.float64 else np.float32)
+
+
+def _typed(t, dtype, name):
+    if t is not None and t.dtype != dtype:
+        raise ValueError(f"{name}: {t.dtype} where {dtype} is needed")
+    return t
+
+
+def _ints(t, size, name):
+    if t is not None and _code(t, _INTS) != size:
+        raise ValueError(f"{name}: {t.dtype} where {8 * size}-bit integers are needed")
+    return t
+
+
+def _int32(t):
+    if _is_torch(t):
+        import torch
+
+        return torch.int32
+    return np.dtype(np.int32)
+
+
+_programs = {}
+
+
+def _program(kernel):
+    """C.kprog, kept for the specs a program calls with again and again"""
+    if isinstance(kernel, C.KProg):
+        return kernel
+    p = _programs.get(kernel)
+    if p is None:
+        if len(_programs) > 64:
+            _programs.clear()
+        p = _programs[kernel] = C.kprog(kernel)
+    return p
+
+
+def _line(t, length, name):
+    """address of a contiguous vector"""
+    if t is None:
+        return None
+    if len(t.shape) != 1 or t.shape[0] != length:
+        raise FriedrichError(C.FR_SHAPE, f"{name}: {tuple(t.shape)} where ({length},) is needed")
+    if length > 1 and _strides(t)[0] != 1:
+        raise ValueError(f"{name}: has to be contiguous")
+    return _address(t)
+
+
 class Context:
     """fr_ctx: one per (process, GPU).  Fails loudly when no gfx950 device / library is present."""
 
@@ -304,6 +432,139 @@ class Context:
         self.check(self.lib.fr_chol_upload_l(self.h, l.ptr, l.rows, l.ld, x.ptr, x.ld, x.cols, int(capacity_hint),
                                              ctypes.byref(h)))
         return Cholesky(self, h)
+
+    # ordered inputs: the gated linear recurrence -------------------------------------------------------
+    def recurrence(self, gate, x, form="log", offsets=None, h0=None, out=None, last=None):
+        """h_t = a_t h_{t-1} + c_t x_t over packed sequences (fr_recurrence).  gate: n x gate_cols, x: n x d, torch tensors or numpy arrays
+        of one type and layout; form: "value" | "log" | "stationary"; offsets: int64 row numbers of the sequences; h0, last: one state per
+        sequence, in the wide type.  -> (h, last): written where given, `last` made where not"""
+        layout = _layout(x, h0, out, gate, last)
+        (n, d), cols, wide = x.shape, gate.shape[1], _wide(x)
+        nseq = 1 if offsets is None else offsets.shape[0] - 1
+        if out is None:
+            out = _like(x, (n, d), layout)
+            if offsets is not None:
+                out[:] = 0  # (rows behind the last sequence stay as they are)
+        if last is None:
+            last = _like(x, (nseq, d), layout, wide)
+        _typed(gate, x.dtype, "gate"), _typed(h0, wide, "h0"), _typed(out, x.dtype, "out"), _typed(last, wide, "last"), _ints(offsets, 8, "offsets")
+        g, xx, s, h, e = (_lead(gate, layout, (n, cols), "gate"), _lead(x, layout, (n, d), "x"), _lead(h0, layout, (nseq, d), "h0"),
+                          _lead(out, layout, (n, d), "out"), _lead(last, layout, (nseq, d), "last"))
+        self.check(self.lib.fr_recurrence(self.h, _code(x), layout, C.GATE_FORMS[form], n, d, g[0], cols, g[1], xx[0], xx[1],
+                                          _line(offsets, nseq + 1, "offsets"), nseq, s[0], s[1], h[0], h[1], e[0], e[1]))
+        return out, last
+
+    def recurrence_backward(self, gate, x, h, dh, form="log", offsets=None, h0=None, dlast=None, dgate=None, dx=None, dh0=None):
+        """gradients of `recurrence` (fr_recurrence_backward) -> (dgate, dx, dh0), written where given and made where not"""
+        layout = _layout(dh, h, h0, dlast, gate, dgate, dx, dh0)
+        (n, d), cols, wide = dh.shape, gate.shape[1], _wide(dh)
+        nseq = 1 if offsets is None else offsets.shape[0] - 1
+        if dgate is None:
+            dgate = _like(gate, (n, cols), layout)
+            if offsets is not None:
+                dgate[:] = 0
+        if dx is None:
+            dx = _like(dh, (n, d), layout)
+            if offsets is not None:
+                dx[:] = 0
+        if dh0 is None:
+            dh0 = _like(dh, (nseq, d), layout, wide)
+        for t, name in ((gate, "gate"), (x, "x"), (h, "h"), (dgate, "dgate"), (dx, "dx")):
+            _typed(t, dh.dtype, name)
+        for t, name in ((h0, "h0"), (dlast, "dlast"), (dh0, "dh0")):
+            _typed(t, wide, name)
+        _ints(offsets, 8, "offsets")
+        big, small = (n, d), (nseq, d)
+        g, xx, s, hh, y, e = (_lead(gate, layout, (n, cols), "gate"), _lead(x, layout, big, "x"), _lead(h0, layout, small, "h0"), _lead(h, layout, big, "h"),
+                              _lead(dh, layout, big, "dh"), _lead(dlast, layout, small, "dlast"))
+        dg, du, ds = _lead(dgate, layout, (n, cols), "dgate"), _lead(dx, layout, big, "dx"), _lead(dh0, layout, small, "dh0")
+        self.check(self.lib.fr_recurrence_backward(self.h, _code(dh), layout, C.GATE_FORMS[form], n, d, g[0], cols, g[1], xx[0], xx[1],
+                                                   _line(offsets, nseq + 1, "offsets"), nseq, s[0], s[1], hh[0], hh[1], y[0], y[1], e[0], e[1], dg[0], dg[1],
+                                                   du[0], du[1], ds[0], ds[1]))
+        return dgate, dx, dh0
+
+    def markov_product(self, kernel, t, V, noise=0.0, out=None):
+        """(K + noise^2 I) V for an Exponential kernel on ordered inputs t (fr_markov_product): gram + gemm in O(n)"""
+        p = C.kprog(kernel)
+        v = _Mat(V)
+        tp, nt, keep = _vecptr(t)
+        if nt != v.rows:
+            raise FriedrichError(C.FR_SHAPE, "inputs and rows differ")
+        if out is None:
+            out = _like(V, (v.rows, v.cols), C.FR_LAYOUT_COLMAJOR) if _is_torch(V) else np.empty((v.rows, v.cols), order="F")
+        o = _Mat(out, writable=True)
+        if (o.rows, o.cols) != (v.rows, v.cols):
+            raise FriedrichError(C.FR_SHAPE, "out has another shape than V")
+        self.check(self.lib.fr_markov_product(self.h, ctypes.byref(p), tp, v.rows, v.ptr, v.cols, v.ld, float(noise), o.ptr, o.ld))
+        return out
+
+    # local experts: the router and their product -----------------------------------------------------------
+    def route(self, logits, k, score="softmax", bias=None, groups=1, top_groups=None, renormalise=True, scale=1.0, experts=None, weights=None, counts=None):
+        """the k best experts of each row and their weights (fr_route) -> (experts int32 n x k, weights n x k in the wide type);
+        counts: int64 per expert, filled if given"""
+        layout = _layout(logits, experts, weights)
+        (n, e), wide = logits.shape, _wide(logits)
+        if experts is None:
+            experts = _like(logits, (n, k), layout, _int32(logits))
+        if weights is None:
+            weights = _like(logits, (n, k), layout, wide)
+        _ints(experts, 4, "experts"), _ints(counts, 8, "counts"), _typed(weights, wide, "weights")
+        if bias is not None and _code(bias) != C.FR_F64:
+            raise ValueError("bias: float64 is needed")
+        z, at, w = _lead(logits, layout, (n, e), "logits"), _lead(experts, layout, (n, k), "experts"), _lead(weights, layout, (n, k), "weights")
+        self.check(self.lib.fr_route(self.h, _code(logits), layout, C.SCORES[score], n, e, z[0], z[1], _line(bias, e, "bias"), groups,
+                                     groups if top_groups is None else top_groups, k, 1 if renormalise else 0, float(scale), at[0], at[1], w[0], w[1],
+                                     _line(counts, e, "counts")))
+        return experts, weights
+
+    def route_backward(self, logits, experts, dweights, score="softmax", renormalise=True, scale=1.0, dlogits=None):
+        """gradient of the weights of `route` in the logits (fr_route_backward) -> dlogits"""
+        layout = _layout(logits, dweights, experts, dlogits)
+        (n, e), k = logits.shape, experts.shape[1]
+        if dlogits is None:
+            dlogits = _like(logits, (n, e), layout)
+        _ints(experts, 4, "experts"), _typed(dweights, _wide(logits), "dweights"), _typed(dlogits, logits.dtype, "dlogits")
+        z, at, w, o = (_lead(logits, layout, (n, e), "logits"), _lead(experts, layout, (n, k), "experts"), _lead(dweights, layout, (n, k), "dweights"),
+                       _lead(dlogits, layout, (n, e), "dlogits"))
+        self.check(self.lib.fr_route_backward(self.h, _code(logits), layout, C.SCORES[score], n, e, z[0], z[1], at[0], at[1], k, 1 if renormalise else 0,
+                                              float(scale), w[0], w[1], o[0], o[1]))
+        return dlogits
+
+    def experts_predict(self, kernel, X, alpha, offsets, Xq, experts, weights, prior_q=None, out=None, slots=None):
+        """means of the query points from the local experts they are routed to (fr_experts_predict) -> (mean, slots); all f64, column-major"""
+        p, col = _program(kernel), C.FR_LAYOUT_COLMAJOR
+        (n, d), (m, k), e = X.shape, experts.shape, offsets.shape[0] - 1
+        if out is None:
+            out = _like(Xq, (m, 1), col)[:, 0]
+        if slots is None:
+            slots = _like(Xq, (m, k), col)
+        for t, name in ((X, "X"), (alpha, "alpha"), (Xq, "Xq"), (weights, "weights"), (prior_q, "prior_q"), (out, "out"), (slots, "slots")):
+            if t is not None and _code(t) != C.FR_F64:
+                raise ValueError(f"{name}: float64 is needed")
+        _ints(experts, 4, "experts"), _ints(offsets, 8, "offsets")
+        x, q, at, w, s = (_lead(X, col, (n, d), "X"), _lead(Xq, col, (m, d), "Xq"), _lead(experts, col, (m, k), "experts"), _lead(weights, col, (m, k), "weights"),
+                          _lead(slots, col, (m, k), "slots"))
+        self.check(self.lib.fr_experts_predict(self.h, ctypes.byref(p), x[0], n, x[1], d, _line(alpha, n, "alpha"), _line(offsets, e + 1, "offsets"), e, q[0], m, q[1],
+                                               at[0], at[1], w[0], w[1], k, _line(prior_q, m, "prior_q"), _line(out, m, "out"), s[0], s[1]))
+        return out, slots
+
+    def experts_backward(self, kernel, X, offsets, Xq, experts, weights, slots, dmean, dweights=None, dalpha=None):
+        """gradients of `experts_predict` in the weights and the coefficients (fr_experts_backward) -> (dweights, dalpha)"""
+        p, col = _program(kernel), C.FR_LAYOUT_COLMAJOR
+        (n, d), (m, k), e = X.shape, experts.shape, offsets.shape[0] - 1
+        if dweights is None:
+            dweights = _like(Xq, (m, k), col)
+        if dalpha is None:
+            dalpha = _like(X, (n, 1), col)[:, 0]
+        for t, name in ((X, "X"), (Xq, "Xq"), (weights, "weights"), (slots, "slots"), (dmean, "dmean"), (dweights, "dweights"), (dalpha, "dalpha")):
+            if _code(t) != C.FR_F64:
+                raise ValueError(f"{name}: float64 is needed")
+        _ints(experts, 4, "experts"), _ints(offsets, 8, "offsets")
+        x, q, at, w, s, dw = (_lead(X, col, (n, d), "X"), _lead(Xq, col, (m, d), "Xq"), _lead(experts, col, (m, k), "experts"), _lead(weights, col, (m, k), "weights"),
+                              _lead(slots, col, (m, k), "slots"), _lead(dweights, col, (m, k), "dweights"))
+        self.check(self.lib.fr_experts_backward(self.h, ctypes.byref(p), x[0], n, x[1], d, _line(offsets, e + 1, "offsets"), e, q[0], m, q[1], at[0], at[1], w[0], w[1], k,
+                                                s[0], s[1], _line(dmean, m, "dmean"), dw[0], dw[1], _line(dalpha, n, "dalpha")))
+        return dweights, dalpha
 
 
 class Cholesky:

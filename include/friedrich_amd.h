@@ -349,6 +349,84 @@ int fr_linear_prior_fit(fr_ctx* ctx, const double* X, int64_t n, int64_t ldx, in
 int fr_grad_terms(fr_chol* chol, const fr_kprog* kernel, const double* y, double noise, int scaled,
                   double* out_grad, double* out_scale);
 
+/* ---- past the cube: ordered inputs and local experts -------------------------------------------------------------------
+ * Operators that answer from models whose covariance matrix is never formed (no reference counterpart: friedrich factors one dense
+ * matrix, algebra/mod.rs:59-92).  They follow the conventions above with these additions:
+ *  - data may be 64, 32 or 16 bits wide (fr_dtype).  Sums, states and weights are 64 bits wide for FR_F64 and 32 bits otherwise;
+ *    that type is called the wide type below.  A 16-bit result is rounded once, to nearest even.
+ *  - a matrix of n rows and c columns is given with its leading dimension in either layout, FR_LAYOUT_COLMAJOR or FR_LAYOUT_ROWMAJOR
+ *    (elements); all matrices of a call share the layout.
+ *  - device pointers have to belong to the context's device; elements are naturally aligned, nothing more is asked of an address.
+ *  - on device data the calls do not wait and may be captured into a HIP graph (fr_ctx_set_stream with the stream that captures).
+ *    A captured call keeps its workspace until the context is destroyed, and takes it from what eager calls left in the context's
+ *    pool: run the same call once before each capture (FR_OUT_OF_MEMORY otherwise).  Host data in a captured call is refused.
+ *  - an output must not overlap an input or another output, except where a call says so. */
+typedef enum { FR_F64 = 0, FR_F32 = 1, FR_BF16 = 2, FR_F16 = 3 } fr_dtype;
+
+/* Gated linear recurrence over packed sequences:  h_t = a_t h_{t-1} + c_t x_t, column by column.
+ *   FR_GATE_VALUE        a = gate,       c = 1
+ *   FR_GATE_LOG          a = exp(gate),  c = 1
+ *   FR_GATE_STATIONARY   a = exp(gate),  c = sqrt(1 - a^2)     (gate <= 0; standard normal x give unit variance for ever)
+ * With gate_i = -(t_i - t_{i-1}) / (2 ls^2) the last one, scaled by sqrt(ampl), is a path of the Exponential kernel's prior
+ * (FR_K_EXPONENTIAL, kernel.rs:661-665) at ordered inputs t.  x and h are n x d, gate is n x gate_cols: gate_cols divides d and each
+ * gate column drives d / gate_cols neighbouring channels.
+ * offsets: nseq + 1 int64 row numbers, in order within [0, n]; sequence s is the rows [offsets[s], offsets[s + 1]), possibly none.  Rows
+ * outside all sequences are neither read for a result nor written.  offsets == NULL: one sequence of n rows (nseq == 1).  Offsets in
+ * device memory are not checked: rows outside [0, n] are never touched, the results of offsets out of order are undefined.
+ * h0 (nseq x d, wide; NULL: zeros) is the state in front of each sequence, h_last (nseq x d, wide; may be NULL) the one behind it -- h0
+ * itself for a sequence without rows.  h may be x, with the same leading dimension. */
+typedef enum { FR_GATE_VALUE = 0, FR_GATE_LOG = 1, FR_GATE_STATIONARY = 2 } fr_gate;
+int fr_recurrence(fr_ctx* ctx, int dtype, int layout, int form, int64_t n, int64_t d, const void* gate, int64_t gate_cols, int64_t ldg,
+                  const void* x, int64_t ldx, const void* offsets, int64_t nseq, const void* h0, int64_t ldh0, void* h, int64_t ldh,
+                  void* h_last, int64_t ldl);
+/* Its backward pass.  h: the forward's output; dh (n x d) and dh_last (nseq x d, wide; NULL: zeros): the gradients that arrive.  dgate
+ * (n x gate_cols, summed over the channels of a gate), dx (n x d), dh0 (nseq x d, wide): the gradients asked for, NULL where not.
+ * x is read for FR_GATE_STATIONARY with dgate only, h with dgate only (NULL otherwise allowed).  Where c_t = 0 (a gate of exactly 1) its
+ * slope is taken as 0.  dx may be dh, with the same leading dimension. */
+int fr_recurrence_backward(fr_ctx* ctx, int dtype, int layout, int form, int64_t n, int64_t d, const void* gate, int64_t gate_cols,
+                           int64_t ldg, const void* x, int64_t ldx, const void* offsets, int64_t nseq, const void* h0, int64_t ldh0,
+                           const void* h, int64_t ldh, const void* dh, int64_t lddh, const void* dh_last, int64_t lddl, void* dgate,
+                           int64_t lddg, void* dx, int64_t lddx, void* dh0, int64_t lddh0);
+/* out (n x m) = (K + noise^2 I) V for a single Exponential kernel on ordered inputs t (n values, t_i <= t_{i+1}), in O(n m): what
+ * fr_gram and fr_gemm give for the n x n matrix, from one recurrence in each direction.  FR_UNSUPPORTED_KERNEL for other programs.  Inputs
+ * out of order: FR_INVALID_ARGUMENT on the host, NaN from device memory. */
+int fr_markov_product(fr_ctx* ctx, const fr_kprog* kernel, const double* t, int64_t n, const double* V, int64_t m, int64_t ldv,
+                      double noise, double* out, int64_t ldo);
+
+/* Routing of n rows to n_experts <= 1024 experts.  Scores of a row's logits: FR_SCORE_SOFTMAX over all experts, or FR_SCORE_SIGMOID
+ * one by one.  An expert of logit -inf is closed to the row.  The experts are ordered by their score + bias (bias: n_experts values; NULL:
+ * by their logits), worked out in 64 bits, of equal ones the lower index first; the bias moves the choice only, never a weight, and a
+ * NaN bias closes its expert.  With n_groups > 1 (<= 64, dividing n_experts: groups of neighbouring experts) only the experts of
+ * the top_groups best groups stay open; a group's value is the sum of its two largest score + bias.  experts (n x k): the k <= 64 best,
+ * best first; weights (n x k, wide): scale times their scores, divided by the scores' sum if renormalise (0 where that sum is 0).  Slots
+ * for which nothing open is left: expert -1, weight 0.  A row with a NaN logit, or under softmax one of +inf: all slots -1, weights NaN.
+ * counts (n_experts int64; may be NULL): how often each expert was chosen. */
+typedef enum { FR_SCORE_SOFTMAX = 0, FR_SCORE_SIGMOID = 1 } fr_score;
+int fr_route(fr_ctx* ctx, int dtype, int layout, int score, int64_t n, int64_t n_experts, const void* logits, int64_t ldl, const double* bias,
+             int64_t n_groups, int64_t top_groups, int64_t k, int renormalise, double scale, int* experts, int64_t lde, void* weights,
+             int64_t ldw, int64_t* counts);
+/* dlogits (n x n_experts) from dweights (n x k, wide) with the choice held fixed.  Slots whose expert lies outside [0, n_experts) take no
+ * part, an expert named twice is counted twice.  Rows without an answer (see above): NaN. */
+int fr_route_backward(fr_ctx* ctx, int dtype, int layout, int score, int64_t n, int64_t n_experts, const void* logits, int64_t ldl,
+                      const void* experts, int64_t lde, int64_t k, int renormalise, double scale, const void* dweights, int64_t lddw,
+                      void* dlogits, int64_t lddl);
+/* Means of m query points from n_experts <= 1024 local models that share a kernel program (f64, column-major like the predict
+ * family).  X (n x d) and alpha (n values: each expert's own K^-1 y) hold the experts' points one expert after the other, expert e has the rows
+ * [offsets[e], offsets[e + 1]) (offsets: n_experts + 1 int64, as in fr_recurrence).  experts (m x k int32), weights (m x k): what
+ * fr_route gives, k <= 64; slots outside [0, n_experts) have a mean of 0.
+ *   out_slots[q, j] = sum_i k(x_q, x_i) alpha_i over the points of experts[q, j]    (m x k; may be NULL)
+ *   out_mean[q]     = prior_q[q] + sum_j weights[q, j] out_slots[q, j]             (prior_q NULL: 0)
+ * One expert with weight 1 is fr_predict_mean with its cached alpha.  The sums' order is fixed by the arguments. */
+int fr_experts_predict(fr_ctx* ctx, const fr_kprog* kernel, const double* X, int64_t n, int64_t ldx, int64_t d, const double* alpha,
+                       const void* offsets, int64_t n_experts, const double* Xq, int64_t m, int64_t ldq, const void* experts, int64_t lde,
+                       const double* weights, int64_t ldw, int64_t k, const double* prior_q, double* out_mean, double* out_slots, int64_t lds);
+/* Its gradients: dweights (m x k) = dmean_q slots[q, j] (slots: the forward's out_slots; read with dweights only), 0 in unused slots; dalpha
+ * (n values) = sum over the slots of the point's expert of dmean_q weights[q, j] k(x_q, x_i), 0 for points of no expert.  NULL: not asked for. */
+int fr_experts_backward(fr_ctx* ctx, const fr_kprog* kernel, const double* X, int64_t n, int64_t ldx, int64_t d, const void* offsets,
+                        int64_t n_experts, const double* Xq, int64_t m, int64_t ldq, const void* experts, int64_t lde, const double* weights,
+                        int64_t ldw, int64_t k, const double* slots, int64_t lds, const double* dmean, double* dweights, int64_t lddw,
+                        double* dalpha);
+
 #ifdef __cplusplus
 }
 #endif

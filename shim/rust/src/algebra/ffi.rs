@@ -47,6 +47,17 @@ pub const FR_LAYOUT_COLMAJOR: c_int = 0;
 pub const FR_LAYOUT_ROWMAJOR: c_int = 1;
 pub const FR_LAYOUT_ROWPTRS: c_int = 2;
 
+// fr_dtype, fr_gate, fr_score
+pub const FR_F64: c_int = 0;
+pub const FR_F32: c_int = 1;
+pub const FR_BF16: c_int = 2;
+pub const FR_F16: c_int = 3;
+pub const FR_GATE_VALUE: c_int = 0;
+pub const FR_GATE_LOG: c_int = 1;
+pub const FR_GATE_STATIONARY: c_int = 2;
+pub const FR_SCORE_SOFTMAX: c_int = 0;
+pub const FR_SCORE_SIGMOID: c_int = 1;
+
 // fr_prof_class
 pub const FR_PROF_GRAM: c_int = 0;
 pub const FR_PROF_POTF2: c_int = 1;
@@ -148,4 +159,34 @@ extern "C" {
     // ---- src/gaussian_process/optimizer.rs
     pub fn fr_grad_terms(chol: *mut fr_chol, kernel: *const fr_kprog, y: *const f64, noise: f64, scaled: c_int,
                          out_grad: *mut f64, out_scale: *mut f64) -> c_int;
+    // ---- past the cube: ordered inputs and local experts
+    pub fn fr_recurrence(ctx: *mut fr_ctx, dtype: c_int, layout: c_int, form: c_int, n: i64, d: i64,
+                         gate: *const c_void, gate_cols: i64, ldg: i64, x: *const c_void, ldx: i64,
+                         offsets: *const c_void, nseq: i64, h0: *const c_void, ldh0: i64, h: *mut c_void, ldh: i64,
+                         h_last: *mut c_void, ldl: i64) -> c_int;
+    pub fn fr_recurrence_backward(ctx: *mut fr_ctx, dtype: c_int, layout: c_int, form: c_int, n: i64, d: i64,
+                                  gate: *const c_void, gate_cols: i64, ldg: i64, x: *const c_void, ldx: i64,
+                                  offsets: *const c_void, nseq: i64, h0: *const c_void, ldh0: i64, h: *const c_void,
+                                  ldh: i64, dh: *const c_void, lddh: i64, dh_last: *const c_void, lddl: i64,
+                                  dgate: *mut c_void, lddg: i64, dx: *mut c_void, lddx: i64, dh0: *mut c_void,
+                                  lddh0: i64) -> c_int;
+    pub fn fr_markov_product(ctx: *mut fr_ctx, kernel: *const fr_kprog, t: *const f64, n: i64, v: *const f64, m: i64,
+                             ldv: i64, noise: f64, out: *mut f64, ldo: i64) -> c_int;
+    pub fn fr_route(ctx: *mut fr_ctx, dtype: c_int, layout: c_int, score: c_int, n: i64, n_experts: i64,
+                    logits: *const c_void, ldl: i64, bias: *const f64, n_groups: i64, top_groups: i64, k: i64,
+                    renormalise: c_int, scale: f64, experts: *mut c_int, lde: i64, weights: *mut c_void, ldw: i64,
+                    counts: *mut i64) -> c_int;
+    pub fn fr_route_backward(ctx: *mut fr_ctx, dtype: c_int, layout: c_int, score: c_int, n: i64, n_experts: i64,
+                             logits: *const c_void, ldl: i64, experts: *const c_void, lde: i64, k: i64,
+                             renormalise: c_int, scale: f64, dweights: *const c_void, lddw: i64, dlogits: *mut c_void,
+                             lddl: i64) -> c_int;
+    pub fn fr_experts_predict(ctx: *mut fr_ctx, kernel: *const fr_kprog, x: *const f64, n: i64, ldx: i64, d: i64,
+                              alpha: *const f64, offsets: *const c_void, n_experts: i64, xq: *const f64, m: i64,
+                              ldq: i64, experts: *const c_void, lde: i64, weights: *const f64, ldw: i64, k: i64,
+                              prior_q: *const f64, out_mean: *mut f64, out_slots: *mut f64, lds: i64) -> c_int;
+    pub fn fr_experts_backward(ctx: *mut fr_ctx, kernel: *const fr_kprog, x: *const f64, n: i64, ldx: i64, d: i64,
+                               offsets: *const c_void, n_experts: i64, xq: *const f64, m: i64, ldq: i64,
+                               experts: *const c_void, lde: i64, weights: *const f64, ldw: i64, k: i64,
+                               slots: *const f64, lds: i64, dmean: *const f64, dweights: *mut f64, lddw: i64,
+                               dalpha: *mut f64) -> c_int;
 }
