@@ -42,6 +42,15 @@ struct DevBuf {
     bool in_use = false;
 };
 
+// a pool buffer that a captured graph works in (typed.hpp: OpWorkspace)
+struct CapturedBuf {
+    void* p;
+    size_t cap;
+    unsigned long long id;  // the capture it was taken in
+    hipStream_t stream;
+    bool busy;  // a call is being captured with it
+};
+
 struct ProfRec {
     hipEvent_t a, b;
     int cls;
@@ -65,6 +74,7 @@ struct fr_ctx {
     std::string err;
     // grow-only workspace pool (stream-ordered reuse inside one context)
     std::vector<fr::DevBuf> pool;
+    std::vector<fr::CapturedBuf> captured;  // buffers of the pool (in_use for good) that captured graphs work in
     // ---- options (fr_ctx_set_option) ----
     int64_t nb = 0;             // outer Cholesky block; 0 = chosen from the matrix size (pick_nb)
     int64_t lookahead = 1;      // the next panel is factored on the panel stream under the trailing update

@@ -1,0 +1,948 @@
+// recur.hpp -- kernels of the gated linear recurrence  h_t = a_t h_{t-1} + c_t x_t  over packed sequences and of its backward pass (one
+// translation unit for each element type includes them; the entry points are in recur.hip).
+//
+// The step is the affine map h -> a h + u; maps compose to maps,  (A2, H2) o (A1, H1) = (A1 A2, A2 H1 + H2),  so a stretch of rows is
+// one pair (A, H) whatever its length.  A row that begins a sequence is the constant map h -> a h0 + u: A = 0 cuts what came before.
+// The gradient runs the other way with the same gates: with Q_t = a_{t+1} G_{t+1} (dh_last behind a sequence's last row),
+//   G_t = dh_t + Q_t,   dx_t = c_t G_t,   da_t = G_t h_{t-1},   Q_{t-1} = a_t G_t,   dh0 = Q in front of the first row.
+// One launch walks everything: a workgroup holds a tile of rows in registers, publishes the tile's map, takes the state in front of the
+// tile from the maps published before it, and writes.
+#pragma once
+
+#include "typed.hpp"
+
+namespace fr {
+
+// workgroups of 256 threads of a kernel that strides over its grid
+inline unsigned blocks_upto(int64_t threads)
+{
+    const int64_t b = (threads + 255) / 256;
+    return (unsigned)(b < 16384 ? b : 16384);
+}
+
+struct RecArgs {
+    int64_t n, d, cols, width, nseq;  // width = d / cols channels share a gate column
+    const int64_t* offsets;           // nseq + 1 row numbers, or null: one sequence of n rows
+    const void *gate, *x, *h0, *hin, *dh, *dlast;
+    void *h, *last, *dgate, *dx, *dh0;
+    // element (t, c) of a matrix lies at t * row + c * col; one of the two is 1
+    int64_t gate_r, gate_c, x_r, x_c, h_r, h_c, dh_r, dh_c, dx_r, dx_c, dg_r, dg_c;
+    int64_t h0_r, h0_c, last_r, last_c, dlast_r, dlast_c, dh0_r, dh0_c;
+    int64_t stretches, tiles;  // runs of rows that one lane walks; workgroups along the rows
+    int64_t blocks, pieces;    // workgroups across the channels; parts that a shared gate's gradient is summed from
+    int lanes;                 // rows layout: log2 of the lanes side by side across the channels
+    int sum_lanes;             // ... lanes whose channels share a gate (0: every channel stores its part)
+    int64_t part_r, part_c;
+    void *ticket, *maps, *carry, *part;
+};
+
+// first row of sequence s, kept inside [0, n] whatever the caller's offsets say
+__device__ __forceinline__ int64_t seq_row(const RecArgs& a, int64_t s)
+{
+    if (!a.offsets) return s == 0 ? 0 : a.n;
+    const int64_t v = a.offsets[s];
+    return v < 0 ? 0 : (v > a.n ? a.n : v);
+}
+
+// the sequence that holds row r (the last one that begins at or before it)
+__device__ __forceinline__ int64_t seq_of(const RecArgs& a, int64_t r)
+{
+    int64_t lo = 0, hi = a.nseq - 1;
+    while (lo < hi) {
+        const int64_t mid = (lo + hi + 1) >> 1;
+        if (seq_row(a, mid) <= r)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    return lo;
+}
+
+// exp(g) and 1 - exp(g) from one polynomial: g = n ln 2 + r with |r| <= 0.3466 (two fused steps), q = exp(r) - 1 by its Taylor series
+// (remainder 0.3466^14 / 14! = 4e-18 in f64, 0.3466^8 / 8! = 5e-9 in f32), exp(g) = 2^n (1 + q).  For n = 0, where 1 - exp(g) would cancel, it
+// is -q itself; elsewhere exp(g) is at most 0.71 or at least 1.41 and the difference is exact to a rounding or two.  Against exp, expm1 and
+// sqrt of the library (about 100 instructions in f64) this is about 45.
+template <typename S>
+struct Exponential {
+    S a, rest;
+};
+__device__ __forceinline__ Exponential<double> exponential(double g)
+{
+    const double n = __builtin_rint(g * 1.44269504088896338700e+00);
+    double r = __builtin_fma(n, -6.93147180369123816490e-01, g);
+    r = __builtin_fma(n, -1.90821492927058770002e-10, r);
+    double p = 1.60590438368216145994e-10;                // 1 / 13!
+    p = __builtin_fma(p, r, 2.08767569878680989792e-09);  // 1 / 12!
+    p = __builtin_fma(p, r, 2.50521083854417187751e-08);
+    p = __builtin_fma(p, r, 2.75573192239858906526e-07);
+    p = __builtin_fma(p, r, 2.75573192239858906526e-06);
+    p = __builtin_fma(p, r, 2.48015873015873015873e-05);
+    p = __builtin_fma(p, r, 1.98412698412698412698e-04);
+    p = __builtin_fma(p, r, 1.38888888888888888889e-03);
+    p = __builtin_fma(p, r, 8.33333333333333333333e-03);
+    p = __builtin_fma(p, r, 4.16666666666666666667e-02);
+    p = __builtin_fma(p, r, 1.66666666666666666667e-01);
+    p = __builtin_fma(p, r, 0.5);
+    const double q = __builtin_fma(p * r, r, r);
+    double a = __builtin_ldexp(1.0 + q, (int)n);
+    a = g < -746.0 ? 0.0 : (g > 710.0 ? __builtin_inf() : a);  // (NaN falls through: r is NaN)
+    return {a, n == 0.0 ? -q : 1.0 - a};
+}
+__device__ __forceinline__ Exponential<float> exponential(float g)
+{
+    const float n = __builtin_rintf(g * 1.44269502f);
+    float r = __builtin_fmaf(n, -6.93145752e-01f, g);
+    r = __builtin_fmaf(n, -1.42860677e-06f, r);
+    float p = 1.98412701e-04f;  // 1 / 7!
+    p = __builtin_fmaf(p, r, 1.38888892e-03f);
+    p = __builtin_fmaf(p, r, 8.33333377e-03f);
+    p = __builtin_fmaf(p, r, 4.16666679e-02f);
+    p = __builtin_fmaf(p, r, 1.66666672e-01f);
+    p = __builtin_fmaf(p, r, 0.5f);
+    const float q = __builtin_fmaf(p * r, r, r);
+    float a = __builtin_ldexpf(1.0f + q, (int)n);
+    a = g < -104.0f ? 0.0f : (g > 89.0f ? __builtin_inff() : a);
+    return {a, n == 0.0f ? -q : 1.0f - a};
+}
+__device__ __forceinline__ double root(double v) { return sqrt(v); }
+__device__ __forceinline__ float root(float v) { return sqrtf(v); }
+
+template <typename S>
+struct Gate {
+    S a, c;
+};
+template <int FORM, typename S>
+__device__ __forceinline__ Gate<S> gate_of(S g)
+{
+    if constexpr (FORM == FR_GATE_VALUE) return {g, S(1)};
+    const Exponential<S> e = exponential(g);
+    if constexpr (FORM == FR_GATE_LOG) return {e.a, S(1)};
+    return {e.a, root(e.rest * (S(1) + e.a))};  // sqrt(1 - a^2) without the cancellation where a is near 1
+}
+// derivative of the row's map with respect to what the caller stores: G h_{t-1} da/dg + G x dc/dg
+template <int FORM, typename S>
+__device__ __forceinline__ S gate_grad(const Gate<S>& g, S G, S before, S x)
+{
+    if constexpr (FORM == FR_GATE_VALUE) return G * before;
+    if constexpr (FORM == FR_GATE_LOG) return G * before * g.a;
+    // c^2 = 1 - e^{2g}: dc/dg = -a^2 / c; a gate of exactly 1 (c = 0) has no finite slope there: taken as 0
+    return g.a * (G * before - (g.c > S(0) ? G * x * g.a / g.c : S(0)));
+}
+
+// ---- what stands in front of a tile ---------------------------------------------------------------------------------------------------
+//
+// Every tile publishes its map as soon as it has read its rows; the state in front of a tile is the state behind the last whole block of
+// tiles (the last tile of a block publishes it) followed by the maps of the block's tiles before it, always in that order: the same
+// bits on every run, whichever tile comes first.  A word is 64 bits and says by itself whether it has been written: all ones, which the
+// workspace is filled with, is a NaN that no result is published as.  So a word needs no flag and no fence beside it.  A tile waits for tiles
+// of lower tickets only, and tickets are drawn by running workgroups: the wait ends, whatever else holds the chip.
+
+// in the place of A: the map ignores what stands in front (NaN patterns that no computed A is published as)
+constexpr unsigned long long kCut = 0x7ff8c07c07c07c07ull;
+constexpr unsigned kCut32 = 0x7fc0c07cu;
+
+constexpr int kRowsWindow = 8;   // tiles in a block, rows layout: each channel reads its own words, so few of them
+constexpr int kRowsOfLane = 8;   // columns layout: rows of a lane (a block is 64 tiles there, one for each lane of a wave)
+// rows layout: rows of a lane; fewer where the data or a gate for each channel take the registers
+template <typename T, bool SHARED>
+constexpr int kRowsOf = SHARED && sizeof(wide_t<T>) == 4 ? 32 : 16;
+
+__device__ __forceinline__ void put_word(unsigned long long* p, unsigned long long w)
+{
+    __hip_atomic_store(p, w == kUnset ? 0x7fffffff7fffffffull : w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ unsigned long long get_word(const unsigned long long* p)
+{
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename S>
+constexpr int kMapWords = sizeof(S) == 8 ? 2 : 1;
+
+__device__ __forceinline__ void put_state(unsigned long long* p, double v) { put_word(p, (unsigned long long)__double_as_longlong(v)); }
+__device__ __forceinline__ void put_state(unsigned long long* p, float v) { put_word(p, __float_as_uint(v)); }
+__device__ __forceinline__ bool get_state(const unsigned long long* p, double& v)
+{
+    const unsigned long long w = get_word(p);
+    v = __longlong_as_double((long long)w);
+    return w != kUnset;
+}
+__device__ __forceinline__ bool get_state(const unsigned long long* p, float& v)
+{
+    const unsigned long long w = get_word(p);
+    v = __uint_as_float((unsigned)w);
+    return w != kUnset;
+}
+constexpr int kPolls = 1 << 22;  // (a bound that a running chip never meets: a wait that met it would leave NaN, not hang)
+
+// the workgroup's tile and channel group: in order of arrival where tiles wait for one another
+__device__ __forceinline__ unsigned claim_tile(const RecArgs& a, unsigned* slot)
+{
+    if (a.tiles == 1) return blockIdx.x;
+    if (threadIdx.x == 0) *slot = atomicAdd((unsigned*)a.ticket, 1u) + 1u;  // (the counter starts from all ones too)
+    __syncthreads();
+    return *slot;
+}
+
+// E neighbouring elements from any address of that element's alignment
+template <typename T, int E>
+struct __attribute__((packed, aligned(sizeof(T)))) Run {
+    T v[E];
+};
+template <typename T, int E>
+__device__ __forceinline__ Run<T, E> load_run(const T* p)
+{
+    Run<T, E> r;
+    __builtin_memcpy(&r, __builtin_assume_aligned(p, sizeof(T)), sizeof(r));
+    return r;
+}
+template <typename T, int E>
+__device__ __forceinline__ void store_run(T* p, const Run<T, E>& r)
+{
+    __builtin_memcpy(__builtin_assume_aligned(p, sizeof(T)), &r, sizeof(r));
+}
+// the map of a stretch of rows; cut: a sequence begins in it, and nothing in front of it counts (an A of 0 would turn an infinite state
+// of the sequence before into a NaN of this one)
+template <typename S>
+struct Map {
+    S A, H;
+    bool cut;
+    __device__ __forceinline__ S of(S state) const { return cut ? H : A * state + H; }
+};
+// first p, then q
+template <typename S>
+__device__ __forceinline__ Map<S> join(const Map<S>& p, const Map<S>& q)
+{
+    return {q.A * p.A, q.of(p.H), p.cut || q.cut};
+}
+template <typename S>
+__device__ __forceinline__ Map<S> shift_up(const Map<S>& m, int step)
+{
+    return {__shfl_up(m.A, step), __shfl_up(m.H, step), (bool)__shfl_up((int)m.cut, step)};
+}
+
+__device__ __forceinline__ void publish(unsigned long long* p, const Map<double>& m)
+{
+    const unsigned long long a = m.cut ? kCut : m.A != m.A ? 0x7ff8000000000000ull : (unsigned long long)__double_as_longlong(m.A);
+    put_word(p, a);
+    put_word(p + 1, (unsigned long long)__double_as_longlong(m.H));
+}
+__device__ __forceinline__ void publish(unsigned long long* p, const Map<float>& m)
+{
+    const unsigned a = m.cut ? kCut32 : m.A != m.A ? 0x7fc00000u : __float_as_uint(m.A);
+    put_word(p, (unsigned long long)a << 32 | __float_as_uint(m.H));
+}
+__device__ __forceinline__ bool published(const unsigned long long* p, Map<double>& m)
+{
+    const unsigned long long a = get_word(p), h = get_word(p + 1);
+    m = {__longlong_as_double((long long)a), __longlong_as_double((long long)h), a == kCut};
+    return a != kUnset && h != kUnset;
+}
+__device__ __forceinline__ bool published(const unsigned long long* p, Map<float>& m)
+{
+    const unsigned long long w = get_word(p);
+    m = {__uint_as_float((unsigned)(w >> 32)), __uint_as_float((unsigned)w), (unsigned)(w >> 32) == kCut32};
+    return w != kUnset;
+}
+
+// Where sequences begin and end among the rows [b, e) of a stretch of R rows from row0 (both lie inside all sequences): bits by steps of the
+// walk, up or down the stretch, and the sequence's number for each such step.  Most stretches lie inside one sequence and end the search with
+// the first look.
+template <int R, bool BACKWARD>
+__device__ __forceinline__ void find_edges(const RecArgs& a, int64_t row0, int64_t b, int64_t e, unsigned& enters, unsigned& leaves, int* number)
+{
+    int64_t s = seq_of(a, b), first = seq_row(a, s), next = seq_row(a, s + 1);
+    for (;;) {
+        const int up = (int)(first - row0), down = (int)(next - 1 - row0);
+        if (first >= b && first < e) {
+            const int i = BACKWARD ? R - 1 - up : up;
+            (BACKWARD ? leaves : enters) |= 1u << i;
+            number[i] = (int)s;
+        }
+        if (next > e || next <= b || next <= first) break;  // (less than b or first: offsets out of order)
+        const int i = BACKWARD ? R - 1 - down : down;
+        (BACKWARD ? enters : leaves) |= 1u << i;
+        number[i] = (int)s;
+        if (next == e) break;
+        first = next;
+        do next = ++s + 1 <= a.nseq ? seq_row(a, s + 1) : a.n + 1;
+        while (next <= first);
+        if (s >= a.nseq) break;
+    }
+}
+
+// ---- rows side by side (FR_LAYOUT_ROWMAJOR) --------------------------------------------------------------------------------------------
+//
+// A lane holds V neighbouring channels of R rows in registers, so the data are read once; 2^lanes lanes stand side by side across the channels,
+// a wave holds 64 >> lanes such stretches of rows and the workgroup's waves the rows after them.
+
+template <typename T, int FORM, int V, bool SHARED, bool BACKWARD>
+__global__ __launch_bounds__(256) void rec_rows_kernel(const RecArgs a)
+{
+    using S = wide_t<T>;
+    constexpr int R = kRowsOf<T, SHARED>;
+    constexpr int BATCH = 8;
+    __shared__ unsigned slot;
+    __shared__ S mapA[4][V][64], mapH[4][V][64], front[V][64];
+    __shared__ int mapC[4][V][64];
+    __shared__ int sequence[V > 1 ? 4 : 256][R];  // of a stretch's rows that begin or end one (V > 1: a wave holds one stretch)
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int across = 1 << a.lanes, cl = lane & (across - 1), group = lane >> a.lanes, groups = 64 >> a.lanes;
+    const unsigned item = claim_tile(a, &slot);
+    const int64_t pos = item / a.blocks;  // tiles in the order of the walk
+    const int64_t c = ((int64_t)(item % a.blocks) * across + cl) * V;
+    const bool live = c < a.d;
+    const int64_t cc = live ? c : 0;
+    const int64_t lo = seq_row(a, 0), hi = seq_row(a, a.nseq);
+    const int64_t stretch = pos * (waves * groups) + wave * groups + group;  // of R rows, in the order of the walk
+    // rows row0 .. row0 + R - 1, walked upwards or downwards; those inside all sequences are [b, e) in steps from the walk's first
+    const int64_t row0 = BACKWARD ? (a.stretches - 1 - stretch) * R : stretch * R;
+    const bool there = stretch < a.stretches;
+    const int64_t rb = lo > row0 ? lo : row0, re = hi < row0 + R ? hi : row0 + R;
+    const bool any = there && live && rb < re;
+    auto row_at = [&](int i) { return BACKWARD ? row0 + (R - 1 - i) : row0 + i; };
+    auto inside = [&](int64_t r) { return any && r >= rb && r < re; };
+    auto address_row = [&](int64_t r) { return r < 0 ? 0 : (r >= a.n ? a.n - 1 : r); };
+
+    const T* __restrict__ gate = (const T*)a.gate + (SHARED ? cc / a.width : cc);
+    const T* __restrict__ in = (const T*)(BACKWARD ? a.dh : a.x) + cc;
+    const int64_t in_r = BACKWARD ? a.dh_r : a.x_r;
+    Run<T, V> raw[R];
+    Run<T, V> graw[SHARED ? 1 : R];
+    S ga[SHARED ? R : 1], gc[SHARED && FORM == FR_GATE_STATIONARY ? R : 1];
+    if (a.n > 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int64_t r = address_row(row_at(i));
+            raw[i] = load_run<T, V>(in + r * in_r);
+            if constexpr (SHARED)
+                ga[i] = widen(gate[r * a.gate_r]);
+            else
+                graw[i] = load_run<T, V>(gate + r * a.gate_r);
+        }
+    }
+    if constexpr (SHARED) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const Gate<S> g = gate_of<FORM, S>(ga[i]);
+            ga[i] = g.a;
+            if constexpr (FORM == FR_GATE_STATIONARY) gc[i] = g.c;
+        }
+    }
+    auto gate_at = [&](int i, int v) -> Gate<S> {
+        if constexpr (SHARED) {
+            if constexpr (FORM == FR_GATE_STATIONARY) return {ga[i], gc[i]};
+            return {ga[i], S(1)};
+        } else
+            return gate_of<FORM, S>(widen(graw[i].v[v]));
+    };
+
+    // steps of the walk that enter a sequence, and steps that leave one
+    unsigned enters = 0, leaves = 0;
+    int* seq = sequence[wave * groups + group];
+    if (any) find_edges<R, BACKWARD>(a, row0, rb, re, enters, leaves, seq);
+    const S* edge = (const S*)(BACKWARD ? a.dlast : a.h0);  // the state a sequence is entered with
+    const int64_t edge_r = BACKWARD ? a.dlast_r : a.h0_r;
+
+    // one row: the state of each channel moves on; returns G (backward) or h (forward)
+    auto step = [&](int i, int v, S state, S& through) -> S {
+        const Gate<S> g = gate_at(i, v);
+        const S u = widen(raw[i].v[v]);
+        if constexpr (BACKWARD) {
+            const S G = u + state;
+            through = g.a * G;
+            return G;
+        } else {
+            const S h = g.a * state + (FORM == FR_GATE_STATIONARY ? g.c * u : u);
+            through = h;
+            return h;
+        }
+    };
+
+    S state[V];
+    if (a.tiles > 1 || groups > 1 || waves > 1) {  // (uniform) the map of the thread's rows, then the state in front of them
+        Map<S> m[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) m[v] = {S(1), S(0), false};
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int64_t r = row_at(i);
+            if (inside(r)) {
+                if (enters >> i & 1) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        m[v].H = edge ? edge[seq[i] * edge_r + c + v] : S(0);
+                        m[v].cut = true;
+                    }
+                }
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    step(i, v, m[v].H, m[v].H);
+                    m[v].A *= gate_at(i, v).a;
+                }
+            }
+        }
+        // across the stretches of the wave (lanes `across` apart), then across the waves
+        Map<S> before[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            for (int d = across; d < 64; d *= 2) {
+                const Map<S> p = shift_up(m[v], d);
+                if (lane >= d) m[v] = join(p, m[v]);
+            }
+            before[v] = shift_up(m[v], across);
+            if (group == 0) before[v] = {S(1), S(0), false};
+            if (group == groups - 1) {
+                mapA[wave][v][cl] = m[v].A;
+                mapH[wave][v][cl] = m[v].H;
+                mapC[wave][v][cl] = m[v].cut;
+            }
+        }
+        __syncthreads();
+        for (int v = wave; v < V; v += waves) {
+            if (lane < across) {
+                const int64_t ch = ((int64_t)(item % a.blocks) * across + lane) * V + v;
+                S st = S(0);
+                if (a.tiles > 1 && ch < a.d) {
+                    Map<S> all = {mapA[0][v][lane], mapH[0][v][lane], mapC[0][v][lane] != 0};
+                    for (int k = 1; k < waves; ++k) all = join(all, Map<S>{mapA[k][v][lane], mapH[k][v][lane], mapC[k][v][lane] != 0});
+                    unsigned long long* words = (unsigned long long*)a.maps;
+                    unsigned long long* states = (unsigned long long*)a.carry;
+                    publish(words + (pos * a.d + ch) * kMapWords<S>, all);
+                    const int64_t block = pos / kRowsWindow, from = block * kRowsWindow;
+                    const int ahead = (int)(pos - from);
+                    Map<S> seen[kRowsWindow - 1];
+                    for (int poll = 0;; ++poll) {
+                        bool ok = block == 0 || get_state(states + (block - 1) * a.d + ch, st);
+#pragma unroll
+                        for (int k = 0; k < kRowsWindow - 1; ++k)
+                            if (k < ahead) ok = published(words + ((from + k) * a.d + ch) * kMapWords<S>, seen[k]) && ok;
+                        if (ok) break;
+                        if (poll == kPolls) {
+                            st = S(NAN);
+                            break;
+                        }
+                        __builtin_amdgcn_s_sleep(1);
+                    }
+#pragma unroll
+                    for (int k = 0; k < kRowsWindow - 1; ++k)
+                        if (k < ahead) st = seen[k].of(st);
+                    if (ahead == kRowsWindow - 1) put_state(states + block * a.d + ch, all.of(st));
+                }
+                front[v][lane] = st;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            S st = front[v][cl];
+            for (int k = 0; k < wave; ++k) st = Map<S>{mapA[k][v][cl], mapH[k][v][cl], mapC[k][v][cl] != 0}.of(st);
+            state[v] = before[v].of(st);
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) state[v] = S(0);
+    }
+
+    // the walk itself
+    if constexpr (!BACKWARD) {
+        T* __restrict__ out = (T*)a.h + cc;
+        S* last = (S*)a.last;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int64_t r = row_at(i);
+            if (inside(r)) {
+                if (enters >> i & 1) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) state[v] = edge ? edge[seq[i] * edge_r + c + v] : S(0);
+                }
+                Run<T, V> y;
+#pragma unroll
+                for (int v = 0; v < V; ++v) y.v[v] = narrow<T>(step(i, v, state[v], state[v]));
+                store_run<T, V>(out + r * a.h_r, y);
+                if (last && (leaves >> i & 1)) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) last[seq[i] * a.last_r + c + v] = state[v];
+                }
+            }
+        }
+        if (last)  // sequences without rows end in the state they began with
+            for (int64_t s0 = pos * (waves * groups) + wave * groups + group; s0 < a.nseq; s0 += a.tiles * (waves * groups))
+                if (live && seq_row(a, s0 + 1) <= seq_row(a, s0))
+#pragma unroll
+                    for (int v = 0; v < V; ++v) last[s0 * a.last_r + c + v] = edge ? edge[s0 * edge_r + c + v] : S(0);
+    } else {
+        const T* __restrict__ hin = (const T*)a.hin + cc;
+        const T* __restrict__ x = (const T*)a.x + cc;
+        const S* h0 = (const S*)a.h0;
+        S* dh0 = (S*)a.dh0;
+        T* __restrict__ dx = (T*)a.dx + cc;
+#pragma unroll
+        for (int i0 = 0; i0 < R; i0 += BATCH) {
+            Run<T, V> hb[BATCH], xb[FORM == FR_GATE_STATIONARY ? BATCH : 1];
+            if (a.dgate && a.n > 0) {
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    hb[i] = load_run<T, V>(hin + address_row(row_at(i0 + i) - 1) * a.h_r);
+                    if constexpr (FORM == FR_GATE_STATIONARY) xb[i] = load_run<T, V>(x + address_row(row_at(i0 + i)) * a.x_r);
+                }
+            }
+            S sum[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const int64_t r = row_at(i0 + i);
+                sum[i] = S(0);
+                if (inside(r)) {
+                    if (enters >> (i0 + i) & 1) {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) state[v] = edge ? edge[seq[i0 + i] * edge_r + c + v] : S(0);
+                    }
+                    const bool first = leaves >> (i0 + i) & 1;
+                    Run<T, V> y, z;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        const S G = step(i0 + i, v, state[v], state[v]);
+                        const Gate<S> g = gate_at(i0 + i, v);
+                        y.v[v] = narrow<T>(FORM == FR_GATE_STATIONARY ? g.c * G : G);
+                        if (a.dgate) {
+                            const S prev = !first ? widen(hb[i].v[v]) : (h0 ? h0[seq[i0 + i] * a.h0_r + c + v] : S(0));
+                            const S dg = gate_grad<FORM, S>(g, G, prev, FORM == FR_GATE_STATIONARY ? widen(xb[FORM == FR_GATE_STATIONARY ? i : 0].v[v]) : S(0));
+                            if constexpr (SHARED) {
+                                sum[i] += dg;
+                                if (a.sum_lanes == 0) ((S*)a.part)[r * a.part_r + (c + v) * a.part_c] = dg;
+                            } else
+                                z.v[v] = narrow<T>(dg);
+                        }
+                    }
+                    if (a.dx) store_run<T, V>(dx + r * a.dx_r, y);
+                    if constexpr (!SHARED)
+                        if (a.dgate) store_run<T, V>((T*)a.dgate + r * a.dg_r + c, z);
+                    if (dh0 && first) {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) dh0[seq[i0 + i] * a.dh0_r + c + v] = state[v];
+                    }
+                }
+            }
+            if constexpr (SHARED) {
+                if (a.dgate && a.sum_lanes > 0) {
+                    for (int d = 1; d < a.sum_lanes; d *= 2)
+#pragma unroll
+                        for (int i = 0; i < BATCH; ++i) sum[i] += __shfl_xor(sum[i], d);
+                    if ((cl & (a.sum_lanes - 1)) == 0) {
+#pragma unroll
+                        for (int i = 0; i < BATCH; ++i) {
+                            const int64_t r = row_at(i0 + i);
+                            if (!inside(r)) continue;
+                            if (a.pieces == 1)
+                                ((T*)a.dgate)[r * a.dg_r + c / a.width] = narrow<T>(sum[i]);
+                            else
+                                ((S*)a.part)[r * a.part_r + c / (64 * V)] = sum[i];
+                        }
+                    }
+                }
+            }
+        }
+        if (dh0)
+            for (int64_t s0 = pos * (waves * groups) + wave * groups + group; s0 < a.nseq; s0 += a.tiles * (waves * groups))
+                if (live && seq_row(a, s0 + 1) <= seq_row(a, s0))
+#pragma unroll
+                    for (int v = 0; v < V; ++v) dh0[s0 * a.dh0_r + c + v] = edge ? edge[s0 * edge_r + c + v] : S(0);
+    }
+}
+
+// ---- columns one after the other (FR_LAYOUT_COLMAJOR) ----------------------------------------------------------------------------------
+//
+// A lane holds E neighbouring rows of up to CG channels that share their gate, a workgroup 64 E rows a wave.  The gate is read, and its
+// exponential worked out, once for those channels.
+
+template <typename T, int FORM, int CG, bool BACKWARD>
+__global__ __launch_bounds__(256) void rec_columns_kernel(const RecArgs a)
+{
+    using S = wide_t<T>;
+    constexpr int E = kRowsOfLane;
+    __shared__ unsigned slot;
+    __shared__ S mapA[CG][4], mapH[CG][4], front[CG];
+    __shared__ int mapC[CG][4];
+    __shared__ int sequence[256][E + 1];  // of a lane's rows that begin or end one (a stride that spreads the banks)
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const unsigned item = claim_tile(a, &slot);
+    const int64_t pos = item / a.blocks;
+    const int64_t block = item % a.blocks, q = block / a.pieces, piece = block % a.pieces;
+    const int64_t c0 = q * a.width + piece * CG;
+    const int ng = (int)(a.width - piece * CG < CG ? a.width - piece * CG : CG);
+    const int64_t lo = seq_row(a, 0), hi = seq_row(a, a.nseq);
+    const int64_t run = pos * blockDim.x + threadIdx.x;  // runs of E rows, in the order of the walk
+    const int64_t row0 = BACKWARD ? (a.stretches - 1 - run) * E : run * E;
+    const bool there = run < a.stretches;
+    const int64_t rb = lo > row0 ? lo : row0, re = hi < row0 + E ? hi : row0 + E;
+    const bool any = there && rb < re;
+    const bool full = any && re - rb == E;
+    // step i of the walk is element at(i) of the run
+    auto at = [](int i) { return BACKWARD ? E - 1 - i : i; };
+
+    auto load = [&](const T* p) {  // E elements of a column from row0; rows that are not there: 0
+        Run<T, E> r;
+        if (there && row0 + E <= a.n)
+            r = load_run<T, E>(p + row0);
+        else
+#pragma unroll
+            for (int i = 0; i < E; ++i) r.v[i] = there && row0 + i < a.n ? p[row0 + i] : narrow<T>(S(0));
+        return r;
+    };
+
+    S ga[E], gc[FORM == FR_GATE_STATIONARY ? E : 1], u[CG][E];
+    {
+        const Run<T, E> g = load((const T*)a.gate + q * a.gate_c);
+        Run<T, E> in[CG];
+#pragma unroll
+        for (int j = 0; j < CG; ++j)
+            if (j < ng) in[j] = load((const T*)(BACKWARD ? a.dh : a.x) + (c0 + j) * (BACKWARD ? a.dh_c : a.x_c));
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const Gate<S> v = gate_of<FORM, S>(widen(g.v[at(i)]));
+            ga[i] = v.a;
+            if constexpr (FORM == FR_GATE_STATIONARY) gc[i] = v.c;
+#pragma unroll
+            for (int j = 0; j < CG; ++j) {
+                u[j][i] = j < ng ? widen(in[j].v[at(i)]) : S(0);
+                if constexpr (FORM == FR_GATE_STATIONARY && !BACKWARD) u[j][i] *= v.c;
+            }
+        }
+    }
+    // rows that enter a sequence (bit i: step i), with the state they enter it with added to their input, and rows that leave one
+    unsigned enters = 0, leaves = 0;
+    unsigned valid = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        if (any && row0 + at(i) >= rb && row0 + at(i) < re) valid |= 1u << i;
+    const S* edge = (const S*)(BACKWARD ? a.dlast : a.h0);
+    const int64_t edge_c = BACKWARD ? a.dlast_c : a.h0_c;
+    int* seq = sequence[threadIdx.x];
+    if (any) find_edges<E, BACKWARD>(a, row0, rb, re, enters, leaves, seq);
+    if (enters && edge) {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (enters >> i & 1)
+#pragma unroll
+                for (int j = 0; j < CG; ++j)
+                    if (j < ng) {
+                        const S h = edge[seq[i] + (c0 + j) * edge_c];
+                        u[j][i] = BACKWARD ? u[j][i] + h : ga[i] * h + u[j][i];
+                    }
+    }
+    // a row's result from the state in front of it, and the state behind it
+    auto step = [&](int i, S in, S state, S& through) -> S {
+        const bool cut = enters >> i & 1;
+        if constexpr (BACKWARD) {
+            const S G = cut ? in : in + state;
+            through = ga[i] * G;
+            return G;
+        } else {
+            const S h = cut ? in : ga[i] * state + in;
+            through = h;
+            return h;
+        }
+    };
+
+    S state[CG], wave_a = S(1);
+    bool wave_cut = false;
+#pragma unroll
+    for (int j = 0; j < CG; ++j) {
+        state[j] = S(0);
+        if (j >= ng) continue;
+        Map<S> m = {S(1), S(0), enters != 0};
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (valid >> i & 1) {
+                step(i, u[j][i], m.H, m.H);
+                m.A *= ga[i];
+            }
+        for (int d = 1; d < 64; d *= 2) {
+            const Map<S> p = shift_up(m, d);
+            if (lane >= d) m = join(p, m);
+        }
+        if (lane == 63) {
+            mapA[j][wave] = m.A;
+            mapH[j][wave] = m.H;
+            mapC[j][wave] = m.cut;
+        }
+        Map<S> before = shift_up(m, 1);
+        if (lane == 0) before = {S(1), S(0), false};
+        // (kept in the place of the state until the workgroup's is known)
+        state[j] = before.H;
+        if (j == 0) {
+            wave_a = before.A;
+            wave_cut = before.cut;
+        }
+    }
+    __syncthreads();
+    for (int j = wave; j < ng; j += waves) {
+        S st = S(0);
+        if (a.tiles > 1) {
+            Map<S> all = {mapA[j][0], mapH[j][0], mapC[j][0] != 0};
+            for (int k = 1; k < waves; ++k) all = join(all, Map<S>{mapA[j][k], mapH[j][k], mapC[j][k] != 0});
+            unsigned long long* words = (unsigned long long*)a.maps;
+            unsigned long long* states = (unsigned long long*)a.carry;
+            const int64_t ch = c0 + j;
+            if (lane == 0) publish(words + (pos * a.d + ch) * kMapWords<S>, all);
+            const int64_t window = pos / 64, from = window * 64;
+            const int ahead = (int)(pos - from);
+            Map<S> m = {S(1), S(0), false};
+            for (int poll = 0;; ++poll) {
+                bool ok = window == 0 || get_state(states + (window - 1) * a.d + ch, st);
+                if (lane < ahead) ok = published(words + ((from + lane) * a.d + ch) * kMapWords<S>, m) && ok;
+                if (__all(ok)) break;
+                if (poll == kPolls) {
+                    st = S(NAN);
+                    break;
+                }
+                __builtin_amdgcn_s_sleep(1);
+            }
+            if (lane >= ahead) m = {S(1), S(0), false};
+            for (int d = 1; d < 64; d *= 2) {
+                const Map<S> p = shift_up(m, d);
+                if (lane >= d) m = join(p, m);
+            }
+            m = {__shfl(m.A, 63), __shfl(m.H, 63), (bool)__shfl((int)m.cut, 63)};
+            st = m.of(st);
+            if (ahead == 63 && lane == 0) put_state(states + window * a.d + ch, all.of(st));
+        }
+        if (lane == 0) front[j] = st;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < CG; ++j) {
+        if (j >= ng) continue;
+        S st = front[j];
+        for (int k = 0; k < wave; ++k) st = Map<S>{mapA[j][k], mapH[j][k], mapC[j][k] != 0}.of(st);
+        state[j] = Map<S>{wave_a, state[j], wave_cut}.of(st);
+    }
+
+    if constexpr (!BACKWARD) {
+        S* last = (S*)a.last;
+#pragma unroll
+        for (int j = 0; j < CG; ++j) {
+            if (j >= ng || !any) continue;
+            T* out = (T*)a.h + (c0 + j) * a.h_c + row0;
+            Run<T, E> y;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                if (valid >> i & 1) {
+                    y.v[at(i)] = narrow<T>(step(i, u[j][i], state[j], state[j]));
+                    if (!full) out[at(i)] = y.v[at(i)];
+                    if (last && (leaves >> i & 1)) last[seq[i] + (c0 + j) * a.last_c] = state[j];
+                }
+            }
+            if (full) store_run<T, E>(out, y);
+        }
+        if (last)
+            for (int64_t s0 = pos * blockDim.x + threadIdx.x; s0 < a.nseq; s0 += a.tiles * blockDim.x)
+                if (seq_row(a, s0 + 1) <= seq_row(a, s0))
+                    for (int j = 0; j < ng; ++j) last[s0 + (c0 + j) * a.last_c] = edge ? edge[s0 + (c0 + j) * edge_c] : S(0);
+    } else {
+        const S* h0 = (const S*)a.h0;
+        S* dh0 = (S*)a.dh0;
+        S dg[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) dg[i] = S(0);
+#pragma unroll
+        for (int j = 0; j < CG; ++j) {
+            if (j >= ng || !any) continue;
+            const int64_t ch = c0 + j;
+            S prev[E];  // of step i: the state in front of its row
+            Run<T, E> xr;
+            if (a.dgate) {
+                const T* hin = (const T*)a.hin + ch * a.h_c + row0 - 1;
+                if (row0 > 0 && row0 + E <= a.n) {
+                    const Run<T, E> hr = load_run<T, E>(hin);
+#pragma unroll
+                    for (int i = 0; i < E; ++i) prev[i] = widen(hr.v[at(i)]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < E; ++i) prev[i] = row0 + at(i) > 0 && row0 + at(i) <= a.n ? widen(hin[at(i)]) : S(0);
+                }
+                if constexpr (FORM == FR_GATE_STATIONARY) xr = load((const T*)a.x + ch * a.x_c);
+            }
+            T* dx = (T*)a.dx + ch * a.dx_c + row0;
+            Run<T, E> y;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                if (valid >> i & 1) {
+                    const S G = step(i, u[j][i], state[j], state[j]);
+                    Gate<S> g = {ga[i], S(1)};
+                    if constexpr (FORM == FR_GATE_STATIONARY) g.c = gc[i];
+                    y.v[at(i)] = narrow<T>(FORM == FR_GATE_STATIONARY ? g.c * G : G);
+                    if (!full && a.dx) dx[at(i)] = y.v[at(i)];
+                    const bool first = leaves >> i & 1;
+                    if (a.dgate) {
+                        const S before = first ? (h0 ? h0[seq[i] + ch * a.h0_c] : S(0)) : prev[i];
+                        S x = S(0);
+                        if constexpr (FORM == FR_GATE_STATIONARY) x = widen(xr.v[at(i)]);
+                        dg[i] += gate_grad<FORM, S>(g, G, before, x);
+                    }
+                    if (dh0 && first) dh0[seq[i] + ch * a.dh0_c] = state[j];
+                }
+            }
+            if (full && a.dx) store_run<T, E>(dx, y);
+        }
+        if (a.dgate && any) {
+            if (a.pieces == 1) {
+                T* out = (T*)a.dgate + q * a.dg_c + row0;
+                Run<T, E> y;
+#pragma unroll
+                for (int i = 0; i < E; ++i) y.v[at(i)] = narrow<T>(dg[i]);
+                if (full)
+                    store_run<T, E>(out, y);
+                else
+#pragma unroll
+                    for (int i = 0; i < E; ++i)
+                        if (valid >> i & 1) out[at(i)] = y.v[at(i)];
+            } else {
+                S* out = (S*)a.part + block * a.part_c + row0;
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if (valid >> i & 1) out[at(i)] = dg[i];
+            }
+        }
+        if (dh0)
+            for (int64_t s0 = pos * blockDim.x + threadIdx.x; s0 < a.nseq; s0 += a.tiles * blockDim.x)
+                if (seq_row(a, s0 + 1) <= seq_row(a, s0))
+                    for (int j = 0; j < ng; ++j) dh0[s0 + (c0 + j) * a.dh0_c] = edge ? edge[s0 + (c0 + j) * edge_c] : S(0);
+    }
+}
+
+// dgate of a shared gate from its parts, in the order of the channels
+template <typename T>
+__global__ __launch_bounds__(256) void rec_heads_kernel(const RecArgs a)
+{
+    using S = wide_t<T>;
+    const int64_t lo = seq_row(a, 0), hi = seq_row(a, a.nseq), step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; id < a.n * a.cols; id += step) {
+        const int64_t r = a.part_r == 1 ? id % a.n : id / a.cols, q = a.part_r == 1 ? id / a.n : id % a.cols;
+        if (r < lo || r >= hi) continue;
+        const S* p = (const S*)a.part + r * a.part_r + q * a.pieces * a.part_c;
+        S sum = S(0);
+        for (int64_t i = 0; i < a.pieces; ++i) sum += p[i * a.part_c];
+        ((T*)a.dgate)[r * a.dg_r + q * a.dg_c] = narrow<T>(sum);
+    }
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------------------------------
+
+// The workgroups along the rows, and the memory that passes states between them (none for a single one)
+template <typename T>
+static int rec_prepare(fr_ctx* ctx, RecArgs& a, int64_t rows, int64_t stretches_of_wave, int64_t window, int64_t parts, OpWorkspace& ws, int* waves)
+{
+    using S = wide_t<T>;
+    a.stretches = (a.n + rows - 1) / rows;
+    int64_t w = (a.stretches + stretches_of_wave - 1) / stretches_of_wave;
+    *waves = (int)(w < 1 ? 1 : (w > 4 ? 4 : w));
+    a.tiles = (a.stretches + *waves * stretches_of_wave - 1) / (*waves * stretches_of_wave);
+    if (a.tiles < 1) a.tiles = 1;
+    if (a.tiles * a.blocks > 0x7fffffffLL / 256 * 64) return set_err(ctx, FR_SHAPE, "%lld rows of %lld channels are too many for one call", (long long)a.n, (long long)a.d);
+    const int64_t maps = a.tiles * a.d * kMapWords<S>, states = (a.tiles / window + 1) * a.d;
+    const int64_t words = a.tiles > 1 ? 1 + maps + states : 0;
+    if (words + parts == 0) return FR_OK;
+    FR_TRY(ws.get((size_t)(words * 8 + parts * (int64_t)sizeof(S))));
+    unsigned long long* p = (unsigned long long*)ws.p;
+    a.ticket = p;
+    a.maps = p + 1;
+    a.carry = p + 1 + maps;
+    a.part = p + words;
+    return words ? launch_unset(ctx, p, words) : FR_OK;
+}
+
+template <typename T, int FORM, int V, bool SHARED>
+static int rec_rows(fr_ctx* ctx, RecArgs& a, bool backward, OpWorkspace& ws)
+{
+    a.lanes = 0;
+    while (a.lanes < 6 && (V << a.lanes) < a.d) ++a.lanes;
+    const int64_t across = 1 << a.lanes, span = across * V;
+    a.blocks = (a.d + span - 1) / span;
+    a.pieces = 1, a.sum_lanes = 0;
+    int64_t parts = 0;
+    if (SHARED && backward && a.dgate) {
+        const int64_t lanes = a.width / V;
+        if (a.cols == 1 && a.blocks == 1)
+            a.sum_lanes = (int)across;
+        else if (a.lanes == 6 && a.width % span == 0)
+            a.sum_lanes = 64, a.pieces = a.width / span;
+        else if (lanes <= across && (lanes & (lanes - 1)) == 0)
+            a.sum_lanes = (int)lanes;
+        else
+            a.pieces = a.width;
+        if (a.pieces > 1) {
+            a.part_r = a.cols * a.pieces, a.part_c = 1;
+            parts = a.n * a.part_r;
+        }
+    }
+    int waves;
+    FR_TRY(rec_prepare<T>(ctx, a, kRowsOf<T, SHARED>, 64 / across, kRowsWindow, parts, ws, &waves));
+    const dim3 grid((unsigned)(a.tiles * a.blocks)), block(64 * waves);
+    if (backward)
+        hipLaunchKernelGGL((rec_rows_kernel<T, FORM, V, SHARED, true>), grid, block, 0, ctx->ls, a);
+    else
+        hipLaunchKernelGGL((rec_rows_kernel<T, FORM, V, SHARED, false>), grid, block, 0, ctx->ls, a);
+    return FR_OK;
+}
+
+template <typename T, int FORM, int CG>
+static int rec_columns(fr_ctx* ctx, RecArgs& a, bool backward, OpWorkspace& ws)
+{
+    a.pieces = (a.width + CG - 1) / CG;
+    a.blocks = a.cols * a.pieces;
+    const bool join = backward && a.dgate && a.pieces > 1;
+    a.part_r = 1, a.part_c = a.n;
+    int waves;
+    FR_TRY(rec_prepare<T>(ctx, a, kRowsOfLane, 64, 64, join ? a.blocks * a.n : 0, ws, &waves));
+    const dim3 grid((unsigned)(a.tiles * a.blocks)), block(64 * waves);
+    if (backward)
+        hipLaunchKernelGGL((rec_columns_kernel<T, FORM, CG, true>), grid, block, 0, ctx->ls, a);
+    else
+        hipLaunchKernelGGL((rec_columns_kernel<T, FORM, CG, false>), grid, block, 0, ctx->ls, a);
+    return FR_OK;
+}
+
+// one row after the other in memory: a single channel of a rows layout is a column
+static bool rec_is_column(const RecArgs& a)
+{
+    return a.d == 1 && a.gate_r == 1 && (!a.x || a.x_r == 1) && (!a.h0 || a.h0_r == 1) && (!a.h || a.h_r == 1) && (!a.last || a.last_r == 1) && (!a.hin || a.h_r == 1) &&
+           (!a.dh || a.dh_r == 1) && (!a.dlast || a.dlast_r == 1) && (!a.dgate || a.dg_r == 1) && (!a.dx || a.dx_r == 1) && (!a.dh0 || a.dh0_r == 1);
+}
+
+template <typename T, int FORM>
+static int rec_launch(fr_ctx* ctx, RecArgs& a, int layout, bool backward, OpWorkspace& ws)
+{
+    constexpr int WIDE = 8 / (int)sizeof(T);  // channels of a lane: 8 bytes of them once that fills a wave
+    if (layout == FR_LAYOUT_COLMAJOR || rec_is_column(a)) {
+        if (a.width == 1)
+            FR_TRY((rec_columns<T, FORM, 1>(ctx, a, backward, ws)));
+        else if (a.width == 2)
+            FR_TRY((rec_columns<T, FORM, 2>(ctx, a, backward, ws)));
+        else
+            FR_TRY((rec_columns<T, FORM, 4>(ctx, a, backward, ws)));
+    } else if (WIDE > 1 && a.d >= 64 * WIDE && a.d % WIDE == 0 && (a.width == 1 || a.width % WIDE == 0)) {
+        if (a.width == 1)
+            FR_TRY((rec_rows<T, FORM, WIDE, false>(ctx, a, backward, ws)));
+        else
+            FR_TRY((rec_rows<T, FORM, WIDE, true>(ctx, a, backward, ws)));
+    } else if (a.width == 1)
+        FR_TRY((rec_rows<T, FORM, 1, false>(ctx, a, backward, ws)));
+    else
+        FR_TRY((rec_rows<T, FORM, 1, true>(ctx, a, backward, ws)));
+    if (backward && a.dgate && a.pieces > 1 && a.n > 0)
+        hipLaunchKernelGGL((rec_heads_kernel<T>), dim3(blocks_upto(a.n * a.cols)), dim3(256), 0, ctx->ls, a);
+    FR_HIP(ctx, hipGetLastError());
+    return FR_OK;
+}
+
+template <typename T>
+int rec_run(fr_ctx* ctx, RecArgs& a, int layout, int form, bool backward, OpWorkspace& ws)
+{
+    switch (form) {
+    case FR_GATE_VALUE: return rec_launch<T, FR_GATE_VALUE>(ctx, a, layout, backward, ws);
+    case FR_GATE_LOG: return rec_launch<T, FR_GATE_LOG>(ctx, a, layout, backward, ws);
+    default: return rec_launch<T, FR_GATE_STATIONARY>(ctx, a, layout, backward, ws);
+    }
+}
+
+}  // namespace fr

@@ -1,0 +1,6 @@
+// recur_f64.hip -- the kernels of recur.hpp for one element type.
+#include "recur.hpp"
+
+namespace fr {
+template int rec_run<double>(fr_ctx*, RecArgs&, int, int, bool, OpWorkspace&);
+}

@@ -3,32 +3,57 @@
 
 namespace fr {
 
-bool stream_capturing(fr_ctx* ctx)
+unsigned long long stream_capture(fr_ctx* ctx)
 {
-    if (!ctx->stream) return false;  // the null stream cannot be captured
+    if (!ctx->stream) return 0;  // the null stream cannot be captured
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(ctx->stream, &st) != hipSuccess) {
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo(ctx->stream, &st, &id) != hipSuccess) {
         (void)hipGetLastError();
-        return false;
+        return 0;
     }
-    return st != hipStreamCaptureStatusNone;
+    return st == hipStreamCaptureStatusNone ? 0 : id + 1;
+}
+
+__global__ __launch_bounds__(256) void unset_kernel(unsigned long long* p, int64_t n)
+{
+    const int64_t step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) p[i] = kUnset;
+}
+
+int launch_unset(fr_ctx* ctx, unsigned long long* p, int64_t n)
+{
+    const int64_t blocks = (n + 255) / 256;
+    hipLaunchKernelGGL(unset_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, ctx->ls, p, n);
+    FR_HIP(ctx, hipGetLastError());
+    return FR_OK;
 }
 
 int OpWorkspace::get(size_t bytes)
 {
-    if (!stream_capturing(ctx)) {
+    const unsigned long long id = stream_capture(ctx);
+    if (!id) {
         p = ws_get(ctx, bytes);
         return p ? FR_OK : FR_OUT_OF_MEMORY;
+    }
+    for (size_t i = 0; i < ctx->captured.size(); ++i) {
+        CapturedBuf& b = ctx->captured[i];
+        if (b.id != id || b.stream != ctx->stream || b.busy || b.cap < bytes) continue;
+        b.busy = true;
+        p = b.p;
+        kept = (int)i;
+        return FR_OK;
     }
     DevBuf* best = nullptr;
     for (DevBuf& b : ctx->pool)
         if (b.p && !b.in_use && b.cap >= bytes && (!best || b.cap < best->cap)) best = &b;
     if (!best)
         return set_err(ctx, FR_OUT_OF_MEMORY,
-                       "a captured call needs a workspace of %zu bytes and cannot allocate it: run the same call once outside the capture before each capture", bytes);
-    best->in_use = true;
+                       "a captured call needs a workspace of %zu bytes and cannot allocate it: run the calls once outside the capture before each capture", bytes);
+    ctx->captured.push_back({best->p, best->cap, id, ctx->stream, true});
+    kept = (int)ctx->captured.size() - 1;
     p = best->p;
-    kept = true;
+    best->in_use = true;
     return FR_OK;
 }
 
@@ -48,7 +73,7 @@ int Operand::stage(const void* p, int64_t line, int64_t lines, int64_t ld_, int6
         dev = (char*)const_cast<void*>(p);
         return FR_OK;
     }
-    if (stream_capturing(ctx)) return set_err(ctx, FR_INVALID_ARGUMENT, "%s: host memory in a captured call", name);
+    if (stream_capture(ctx)) return set_err(ctx, FR_INVALID_ARGUMENT, "%s: host memory in a captured call", name);
     ld = line;
     FR_TRY(ws.get((size_t)(elem * line * lines)));
     dev = (char*)ws.p;

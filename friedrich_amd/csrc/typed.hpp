@@ -56,21 +56,25 @@ __device__ __forceinline__ __hip_bfloat16 narrow<__hip_bfloat16>(float v)
 inline int64_t dtype_size(int dtype) { return dtype == FR_F64 ? 8 : dtype == FR_F32 ? 4 : 2; }
 inline int64_t wide_size(int dtype) { return dtype == FR_F64 ? 8 : 4; }
 
-// the call's stream is being captured into a graph: no allocation, no copy to or from pageable memory, no wait
-bool stream_capturing(fr_ctx* ctx);
+// the capture that the call's stream is in, 0 if none: there is no allocation, no copy to or from pageable memory and no wait in one
+unsigned long long stream_capture(fr_ctx* ctx);
 
 // A workspace for one call.  Eager calls take it from the context's pool and give it back (the pool is stream-ordered).  A captured
-// call keeps it for as long as the context lives: a graph is replayed on any stream, next to other graphs and to eager calls of the
-// context, so nothing else may ever be handed the same bytes.
+// call takes it out of the pool for as long as the context lives: a graph is replayed on any stream, next to other graphs and to eager calls
+// of the context, so nobody else may be handed the same bytes.  Only later calls of the same capture on the same stream, which its replays
+// run one after the other, use it again.
 struct OpWorkspace {
     fr_ctx* ctx;
     void* p = nullptr;
-    bool kept = false;
+    int kept = -1;  // its place in ctx->captured
     explicit OpWorkspace(fr_ctx* c) : ctx(c) {}
     OpWorkspace(const OpWorkspace&) = delete;
     ~OpWorkspace()
     {
-        if (p && !kept) ws_put(ctx, p);
+        if (kept >= 0)
+            ctx->captured[kept].busy = false;
+        else if (p)
+            ws_put(ctx, p);
     }
     int get(size_t bytes);
 };
@@ -97,6 +101,11 @@ private:
     char* host = nullptr;
     int64_t host_ld = 0, line_ = 0, lines_ = 0, elem_ = 0;
 };
+
+// 64-bit words that no kernel has written yet, between workgroups that pass results on (not hipMemsetAsync: such nodes of a captured graph
+// have given wrong results on replays)
+constexpr unsigned long long kUnset = ~0ull;
+int launch_unset(fr_ctx* ctx, unsigned long long* p, int64_t n);
 
 // The contiguous axis first: (line, lines) of a rows x cols matrix in a layout
 inline int stage_matrix(Operand& o, int layout, const void* p, int64_t rows, int64_t cols, int64_t ld, int64_t elem, const char* name, bool output = false)

@@ -264,6 +264,38 @@ def test_gates_of_zero_one_and_beyond(tctx):
     assert torch.isfinite(dg).all() and torch.equal(dx, 0 * dx) and float(dh0) == n
 
 
+@pytest.mark.parametrize("layout", ["row", "col"])
+def test_what_is_not_finite_stays_in_its_sequence(tctx, layout):
+    """a NaN or an infinity reaches the later rows of its own sequence (the earlier ones in the gradient) and no other"""
+    import torch
+
+    rng = np.random.default_rng(14)
+    for dtype in ("f64", "f32", "bf16"):
+        for d in (2, 300):
+            cuts = [0, 5, 700, 701, 2500, 2600, 5000]
+            n, nseq = cuts[-1], len(cuts) - 1
+            gate, x, h0, wide = problem(rng, n, d, d, nseq, "log", dtype, layout)
+            offsets = torch.tensor(cuts, dtype=torch.int64, device="cuda")
+            clean, clean_last = tctx.recurrence(gate, x, offsets=offsets, h0=h0)
+            dh = put(rng.standard_normal((n, d)), layout, x.dtype)
+            clean_dx = tctx.recurrence_backward(gate, None, clean, dh, offsets=offsets, h0=h0)[1].clone()
+            for value in (float("nan"), float("inf")):
+                for row in (4, 300, 700, 2499, 4000):
+                    s = max(i for i, c in enumerate(cuts) if c <= row)
+                    x2, dh2 = x.clone(), dh.clone()
+                    x2[row], dh2[row] = value, value
+                    h, last = tctx.recurrence(gate, x2, offsets=offsets, h0=h0)
+                    touched = torch.zeros(n, dtype=torch.bool, device="cuda")
+                    touched[row:cuts[s + 1]] = True
+                    assert torch.equal(h[~touched], clean[~touched]) and not torch.isfinite(h[row:cuts[s + 1]]).any(), (dtype, d, row)
+                    other = [i for i in range(nseq) if i != s]
+                    assert torch.equal(last[other], clean_last[other])
+                    dx = tctx.recurrence_backward(gate, None, clean, dh2, offsets=offsets, h0=h0)[1]
+                    touched[:] = False
+                    touched[cuts[s]:row + 1] = True
+                    assert torch.equal(dx[~touched], clean_dx[~touched]) and not torch.isfinite(dx[cuts[s]:row + 1]).any(), (dtype, d, row)
+
+
 def test_host_arrays(tctx):
     rng = np.random.default_rng(8)
     for order in ("F", "C"):
