@@ -348,6 +348,9 @@ def test_refusals(tctx):  # noqa: F811
         with pytest.raises(FriedrichError) as e:
             tctx.experts_predict(("squared_exp", 1.0, 1.0), X, alpha, np.array(bad, dtype=np.int64), Xq, chosen, w)
         assert e.value.status == C.FR_SHAPE
+    with pytest.raises(FriedrichError) as e:
+        tctx.experts_predict(("squared_exp", 1.0, 1.0), X[:, :0], alpha, offsets, Xq[:, :0], chosen, w)
+    assert e.value.status == C.FR_SHAPE
     with pytest.raises(FriedrichError):
         tctx.experts_predict(("squared_exp", 1.0, 1.0), X, alpha, np.zeros(1026, dtype=np.int64), Xq, chosen, w)
     with pytest.raises(FriedrichError):
