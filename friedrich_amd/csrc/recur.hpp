@@ -183,23 +183,6 @@ __device__ __forceinline__ unsigned claim_tile(const RecArgs& a, unsigned* slot)
     return *slot;
 }
 
-// E neighbouring elements from any address of that element's alignment
-template <typename T, int E>
-struct __attribute__((packed, aligned(sizeof(T)))) Run {
-    T v[E];
-};
-template <typename T, int E>
-__device__ __forceinline__ Run<T, E> load_run(const T* p)
-{
-    Run<T, E> r;
-    __builtin_memcpy(&r, __builtin_assume_aligned(p, sizeof(T)), sizeof(r));
-    return r;
-}
-template <typename T, int E>
-__device__ __forceinline__ void store_run(T* p, const Run<T, E>& r)
-{
-    __builtin_memcpy(__builtin_assume_aligned(p, sizeof(T)), &r, sizeof(r));
-}
 // the map of a stretch of rows; cut: a sequence begins in it, and nothing in front of it counts (an A of 0 would turn an infinite state
 // of the sequence before into a NaN of this one)
 template <typename S>

@@ -53,6 +53,23 @@ __device__ __forceinline__ __hip_bfloat16 narrow<__hip_bfloat16>(float v)
     return r;
 }
 
+// E neighbouring elements from any address of that element's alignment
+template <typename T, int E>
+struct __attribute__((packed, aligned(sizeof(T)))) Run {
+    T v[E];
+};
+template <typename T, int E>
+__device__ __forceinline__ Run<T, E> load_run(const T* p)
+{
+    Run<T, E> r;
+    __builtin_memcpy(&r, __builtin_assume_aligned(p, sizeof(T)), sizeof(r));
+    return r;
+}
+template <typename T, int E>
+__device__ __forceinline__ void store_run(T* p, const Run<T, E>& r)
+{
+    __builtin_memcpy(__builtin_assume_aligned(p, sizeof(T)), &r, sizeof(r));
+}
 inline int64_t dtype_size(int dtype) { return dtype == FR_F64 ? 8 : dtype == FR_F32 ? 4 : 2; }
 inline int64_t wide_size(int dtype) { return dtype == FR_F64 ? 8 : 4; }
 

@@ -47,6 +47,66 @@ def test_route(tctx, score, dtype, layout):  # noqa: F811
             assert np.array_equal(counts.cpu().numpy(), want_c)
 
 
+def test_route_many_rows(tctx):  # noqa: F811
+    """the way of many rows: keys in 32 bits, rows that they do not decide in 64 -- ties of logits, of logits with a bias, biases that differ in
+    their last bits only, values whose scores saturate, groups that are alike; choices checked against 64-bit scores by sorting"""
+    import torch
+
+    rng = np.random.default_rng(30)
+    n = 20000
+    for i, (experts, k, groups, kept, dtype, score) in enumerate([(256, 8, 8, 4, "f32", "sigmoid"), (64, 2, 1, 1, "bf16", "softmax"), (100, 5, 1, 1, "f64", "sigmoid"),
+                                                                  (32, 8, 4, 2, "bf16", "sigmoid"), (512, 6, 1, 1, "f32", "softmax"), (16, 1, 2, 1, "f16", "softmax")]):
+        z = rng.standard_normal((n, experts)) * np.where(np.arange(n) % 3 == 0, 0.0, np.where(np.arange(n) % 3 == 1, 2.0, 20.0))[:, None]
+        z[5::7] = np.round(z[5::7])  # ties
+        z[rng.random((n, experts)) < 0.02] = -np.inf
+        z[11], z[12, 3] = -np.inf, np.nan
+        flat = np.zeros(experts)
+        close = 0.25 + 2.0**-40 * rng.integers(0, 4, experts)
+        for bias in (None, flat, close, 0.1 * rng.standard_normal(experts)):
+            for layout in ("row", "col"):
+                logits = put(z, layout, torch_types()[dtype])
+                b = None if bias is None else torch.from_numpy(bias).cuda()
+                counts = torch.zeros(experts, dtype=torch.int64, device="cuda")
+                got, w = tctx.route(logits, k, score=score, bias=b, groups=groups, top_groups=kept, renormalise=bool(i & 1), scale=1.5, counts=counts)
+                x = host(logits)
+                bad = np.isnan(x).any(1)
+                p = P.scores(score, np.where(np.isnan(x), 0.0, x))
+                rank = p + (0.0 if bias is None else bias)
+                rank[np.isneginf(x)] = -np.inf
+                key = np.where(np.isneginf(x), -np.inf, x if bias is None else rank)
+                if kept < groups:
+                    two = -np.sort(-rank.reshape(n, groups, -1), axis=2)[:, :, :2]
+                    value = two[:, :, 0] + np.where(np.isneginf(two[:, :, 1]), 0.0, two[:, :, 1])
+                    best = np.argsort(-value, axis=1, kind="stable")[:, :kept]
+                    open_ = np.zeros((n, groups), bool)
+                    np.put_along_axis(open_, best, True, 1)
+                    key = np.where(np.repeat(open_, experts // groups, axis=1), key, -np.inf)
+                order = np.argsort(-key, axis=1, kind="stable")[:, :k]
+                want = np.where(np.isneginf(np.take_along_axis(key, order, 1)), -1, order)
+                want[bad] = -1
+                same = (got.cpu().numpy() == want).all(1)
+                # numpy's exponential and the kernel's differ by an ulp: rows whose deciding 64-bit keys lie within 4 ulp may differ
+                lead = -np.sort(-np.where(np.isneginf(key), -1e300, key), axis=1)[:, :k + 1]
+                with np.errstate(invalid="ignore"):
+                    gaps = lead[:, :-1] - lead[:, 1:]
+                tight = ((gaps > 0) & (gaps < 1e-15 * (1 + np.abs(lead[:, :-1])))).any(1) if bias is not None else np.zeros(n, bool)
+                if kept < groups:
+                    v = -np.sort(-value, axis=1)
+                    tight |= (v[:, kept - 1] - v[:, kept] < 1e-15 * 4) & (v[:, kept - 1] != v[:, kept])
+                assert (same | tight).all(), (i, layout, bias is None, int((~(same | tight)).sum()))
+                chosen = np.where(want < 0, 0, want)
+                ww = np.where(want < 0, 0.0, np.take_along_axis(p, chosen, 1))
+                if i & 1:
+                    total = ww.sum(1, keepdims=True)
+                    ww = np.where(total > 0, ww / np.where(total > 0, total, 1.0), 0.0)
+                ww = 1.5 * ww
+                ok = same & ~bad
+                assert np.all((np.abs(host(w) - ww) <= weights_bound(dtype, experts, k, ww, bool(i & 1)))[ok])
+                assert np.isnan(host(w)[bad]).all()
+                c = got.cpu().numpy()
+                assert np.array_equal(counts.cpu().numpy(), np.bincount(c[c >= 0], minlength=experts))
+
+
 def test_route_ties_masks_and_rows_without_an_answer(tctx):  # noqa: F811
     import torch
 
