@@ -9,6 +9,8 @@
 // tile from the maps published before it, and writes.
 #pragma once
 
+#include <type_traits>
+
 #include "typed.hpp"
 
 namespace fr {
@@ -141,11 +143,16 @@ __device__ __forceinline__ S gate_grad(const Gate<S>& g, S G, S before, S x)
 constexpr unsigned long long kCut = 0x7ff8c07c07c07c07ull;
 constexpr unsigned kCut32 = 0x7fc0c07cu;
 
-constexpr int kRowsWindow = 8;   // tiles in a block, rows layout: each channel reads its own words, so few of them
-constexpr int kRowsOfLane = 8;   // columns layout: rows of a lane (a block is 64 tiles there, one for each lane of a wave)
-// rows layout: rows of a lane; fewer where the data or a gate for each channel take the registers
-template <typename T, bool SHARED>
-constexpr int kRowsOf = SHARED && sizeof(wide_t<T>) == 4 ? 32 : 16;
+constexpr int kRowsWindow = 16;    // tiles in a block, rows layout: a lane reads the words of its own channel, so few of them
+constexpr int kColumnsWindow = 64;  // ... columns layout: one for each lane of a wave
+constexpr int kRowsOfLane = 8;      // columns layout: rows of a lane
+constexpr int kWaves = 8;           // of a workgroup, at most
+constexpr int64_t kFewRows = 1024;  // rows layout, forward: up to here 4 rows a lane
+// rows layout: rows of a lane; fewer where the data, a gate for each channel, a second factor of a row or the backward pass's second operand take
+// the registers (backward, bf16, 16413 x 2048: 83 us with 16 rows, 106 with 32; forward 61 and 58).  FEW: calls of
+// a few rows, where the unrolled walk of 16 spends its time fetching instructions
+template <typename T, int FORM, bool SHARED, bool UNIFORM, bool BACKWARD, bool FEW>
+constexpr int kRowsOf = FEW ? 4 : UNIFORM && SHARED && !BACKWARD && FORM != FR_GATE_STATIONARY && sizeof(wide_t<T>) == 4 ? 32 : 16;
 
 __device__ __forceinline__ void put_word(unsigned long long* p, unsigned long long w)
 {
@@ -231,9 +238,14 @@ __device__ __forceinline__ bool published(const unsigned long long* p, Map<float
 // walk, up or down the stretch, and the sequence's number for each such step.  Most stretches lie inside one sequence and end the search with
 // the first look.
 template <int R, bool BACKWARD>
-__device__ __forceinline__ void find_edges(const RecArgs& a, int64_t row0, int64_t b, int64_t e, unsigned& enters, unsigned& leaves, int* number)
+__device__ __forceinline__ void find_edges(const RecArgs& a, int64_t lo, int64_t hi, int64_t row0, int64_t b, int64_t e, unsigned& enters, unsigned& leaves, int* number)
 {
-    int64_t s = seq_of(a, b), first = seq_row(a, s), next = seq_row(a, s + 1);
+    int64_t s = 0, first = lo, next = hi;  // (the rows of all sequences: those of the only one)
+    if (a.nseq > 1) {
+        s = seq_of(a, b);
+        first = seq_row(a, s);
+        next = seq_row(a, s + 1);
+    }
     for (;;) {
         const int up = (int)(first - row0), down = (int)(next - 1 - row0);
         if (first >= b && first < e) {
@@ -253,41 +265,92 @@ __device__ __forceinline__ void find_edges(const RecArgs& a, int64_t row0, int64
     }
 }
 
+// For a whole wave, rows [b, e) the same in every lane: `base` is the sequence that holds row b, lane l gets the first row of sequence base + l
+// (beyond the last sequence: a row that is never reached).  64 offsets a look: two looks for 4096 sequences.
+__device__ __forceinline__ int64_t wave_sequences(const RecArgs& a, int64_t b, int64_t& base)
+{
+    const int lane = threadIdx.x & 63;
+    int64_t span = a.nseq;
+    base = 0;
+    while (span > 1) {
+        const int64_t stride = (span + 63) >> 6, i = base + lane * stride;
+        const int64_t v = seq_row(a, i < base + span ? i : base);
+        const int below = __popcll(__ballot(i < base + span && v <= b));
+        const int64_t skip = (below > 0 ? below - 1 : 0) * stride;
+        base += skip;
+        span = span - skip < stride ? span - skip : stride;
+    }
+    const int64_t v = seq_row(a, base + lane <= a.nseq ? base + lane : a.nseq);
+    return base + lane <= a.nseq ? v : a.n + 1;
+}
+// whether a sequence begins or ends among the rows; many: in more places than a wave holds
+__device__ __forceinline__ bool wave_edges(int64_t first, int64_t b, int64_t e, bool& many)
+{
+    many = __shfl(first, 63) <= e;
+    return __any(first >= b && first <= e);
+}
+// find_edges for a whole wave
+template <int R, bool BACKWARD>
+__device__ __forceinline__ void find_wave_edges(const RecArgs& a, int64_t lo, int64_t hi, int64_t row0, int64_t b, int64_t e, unsigned& enters, unsigned& leaves, int* number)
+{
+    if (a.nseq <= 1) {
+        find_edges<R, BACKWARD>(a, lo, hi, row0, b, e, enters, leaves, number);
+        return;
+    }
+    int64_t base;
+    const int64_t first = wave_sequences(a, b, base);
+    bool many;
+    if (!wave_edges(first, b, e, many)) return;
+    if (many) {
+        find_edges<R, BACKWARD>(a, lo, hi, row0, b, e, enters, leaves, number);
+        return;
+    }
+#pragma unroll 1
+    for (int64_t r = b; r < e; ++r) {
+        const int up = (int)(r - row0), i = BACKWARD ? R - 1 - up : up;
+        const bool begins = __any(first == r), ends = __any(first == r + 1);
+        if (begins) (BACKWARD ? leaves : enters) |= 1u << i;
+        if (ends) (BACKWARD ? enters : leaves) |= 1u << i;
+        if (begins || ends) number[i] = (int)(base + __popcll(__ballot(first <= r)) - 1);
+    }
+}
+
 // ---- rows side by side (FR_LAYOUT_ROWMAJOR) --------------------------------------------------------------------------------------------
 //
 // A lane holds V neighbouring channels of R rows in registers, so the data are read once; 2^lanes lanes stand side by side across the channels,
-// a wave holds 64 >> lanes such stretches of rows and the workgroup's waves the rows after them.
+// a wave holds 64 >> lanes such stretches of rows and the workgroup's waves the rows after them.  UNIFORM: a wave holds one stretch
+// (64 channel lanes), so rows, their addresses and what begins and ends in them are the same for the whole wave and cost no vector
+// instruction; a stretch inside one sequence then runs without a branch.
 
-template <typename T, int FORM, int V, bool SHARED, bool BACKWARD>
-__global__ __launch_bounds__(256) void rec_rows_kernel(const RecArgs a)
+template <typename T, int FORM, int V, bool SHARED, bool BACKWARD, bool UNIFORM, bool FEW>
+__global__ __launch_bounds__(512) void rec_rows_kernel(const RecArgs a)
 {
     using S = wide_t<T>;
-    constexpr int R = kRowsOf<T, SHARED>;
-    constexpr int BATCH = 8;
+    constexpr int R = kRowsOf<T, FORM, SHARED, UNIFORM, BACKWARD, FEW>;
+    constexpr int BATCH = R < 8 ? R : 8;
     __shared__ unsigned slot;
-    __shared__ S mapA[4][V][64], mapH[4][V][64], front[V][64];
-    __shared__ int mapC[4][V][64];
-    __shared__ int sequence[V > 1 ? 4 : 256][R];  // of a stretch's rows that begin or end one (V > 1: a wave holds one stretch)
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int across = 1 << a.lanes, cl = lane & (across - 1), group = lane >> a.lanes, groups = 64 >> a.lanes;
-    const unsigned item = claim_tile(a, &slot);
-    const int64_t pos = item / a.blocks;  // tiles in the order of the walk
-    const int64_t c = ((int64_t)(item % a.blocks) * across + cl) * V;
+    __shared__ S mapA[kWaves][V][64], mapH[kWaves][V][64], front[V][64];
+    __shared__ int mapC[kWaves][V][64];
+    __shared__ int sequence[UNIFORM ? kWaves : kWaves * 64][R];  // of a stretch's rows that begin or end one
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int across = UNIFORM ? 64 : 1 << a.lanes, cl = UNIFORM ? lane : lane & (across - 1), group = UNIFORM ? 0 : lane >> a.lanes, groups = UNIFORM ? 1 : 64 >> a.lanes;
+    const unsigned item = __builtin_amdgcn_readfirstlane(claim_tile(a, &slot));
+    const int64_t pos = item / (unsigned)a.blocks;  // tiles in the order of the walk
+    const unsigned c = ((item % (unsigned)a.blocks) * across + cl) * V;
     const bool live = c < a.d;
-    const int64_t cc = live ? c : 0;
+    const unsigned cc = live ? c : 0;
     const int64_t lo = seq_row(a, 0), hi = seq_row(a, a.nseq);
     const int64_t stretch = pos * (waves * groups) + wave * groups + group;  // of R rows, in the order of the walk
-    // rows row0 .. row0 + R - 1, walked upwards or downwards; those inside all sequences are [b, e) in steps from the walk's first
+    // rows row0 .. row0 + R - 1, walked upwards or downwards; those inside all sequences are [rb, re)
     const int64_t row0 = BACKWARD ? (a.stretches - 1 - stretch) * R : stretch * R;
-    const bool there = stretch < a.stretches;
     const int64_t rb = lo > row0 ? lo : row0, re = hi < row0 + R ? hi : row0 + R;
-    const bool any = there && live && rb < re;
+    const bool any = stretch < a.stretches && rb < re;
     auto row_at = [&](int i) { return BACKWARD ? row0 + (R - 1 - i) : row0 + i; };
-    auto inside = [&](int64_t r) { return any && r >= rb && r < re; };
     auto address_row = [&](int64_t r) { return r < 0 ? 0 : (r >= a.n ? a.n - 1 : r); };
 
-    const T* __restrict__ gate = (const T*)a.gate + (SHARED ? cc / a.width : cc);
-    const T* __restrict__ in = (const T*)(BACKWARD ? a.dh : a.x) + cc;
+    const T* gate = (const T*)a.gate;
+    const unsigned gc0 = SHARED ? cc / (unsigned)a.width : cc;
+    const T* in = (const T*)(BACKWARD ? a.dh : a.x);
     const int64_t in_r = BACKWARD ? a.dh_r : a.x_r;
     Run<T, V> raw[R];
     Run<T, V> graw[SHARED ? 1 : R];
@@ -296,11 +359,11 @@ __global__ __launch_bounds__(256) void rec_rows_kernel(const RecArgs a)
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int64_t r = address_row(row_at(i));
-            raw[i] = load_run<T, V>(in + r * in_r);
+            raw[i] = load_run<T, V>(in + r * in_r + cc);
             if constexpr (SHARED)
-                ga[i] = widen(gate[r * a.gate_r]);
+                ga[i] = widen((gate + r * a.gate_r)[gc0]);
             else
-                graw[i] = load_run<T, V>(gate + r * a.gate_r);
+                graw[i] = load_run<T, V>(gate + r * a.gate_r + gc0);
         }
     }
     if constexpr (SHARED) {
@@ -319,25 +382,36 @@ __global__ __launch_bounds__(256) void rec_rows_kernel(const RecArgs a)
             return gate_of<FORM, S>(widen(graw[i].v[v]));
     };
 
-    // steps of the walk that enter a sequence, and steps that leave one
-    unsigned enters = 0, leaves = 0;
+    // steps of the walk that are rows of a sequence, that enter one, and that leave one
+    unsigned valid = 0, enters = 0, leaves = 0;
     int* seq = sequence[wave * groups + group];
-    if (any) find_edges<R, BACKWARD>(a, row0, rb, re, enters, leaves, seq);
+    if (any) {
+        const int first = BACKWARD ? (int)(row0 + R - re) : (int)(rb - row0), count = (int)(re - rb);
+        valid = (count >= 32 ? ~0u : (1u << count) - 1u) << first;
+        if constexpr (UNIFORM)
+            find_wave_edges<R, BACKWARD>(a, lo, hi, row0, rb, re, enters, leaves, seq);
+        else
+            find_edges<R, BACKWARD>(a, lo, hi, row0, rb, re, enters, leaves, seq);
+    }
+    if constexpr (UNIFORM) {
+        valid = __builtin_amdgcn_readfirstlane(valid);
+        enters = __builtin_amdgcn_readfirstlane(enters);
+        leaves = __builtin_amdgcn_readfirstlane(leaves);
+    }
+    constexpr unsigned ALL = R == 32 ? ~0u : (1u << (R & 31)) - 1u;
+    const bool plain = UNIFORM && valid == ALL && (enters | leaves) == 0;
     const S* edge = (const S*)(BACKWARD ? a.dlast : a.h0);  // the state a sequence is entered with
     const int64_t edge_r = BACKWARD ? a.dlast_r : a.h0_r;
 
-    // one row: the state of each channel moves on; returns G (backward) or h (forward)
-    auto step = [&](int i, int v, S state, S& through) -> S {
-        const Gate<S> g = gate_at(i, v);
-        const S u = widen(raw[i].v[v]);
+    // one row: the state of a channel moves on; returns G (backward) or h (forward)
+    auto step = [&](const Gate<S>& g, S u, S& state) -> S {
         if constexpr (BACKWARD) {
             const S G = u + state;
-            through = g.a * G;
+            state = g.a * G;
             return G;
         } else {
-            const S h = g.a * state + (FORM == FR_GATE_STATIONARY ? g.c * u : u);
-            through = h;
-            return h;
+            state = g.a * state + (FORM == FR_GATE_STATIONARY ? g.c * u : u);
+            return state;
         }
     };
 
@@ -346,34 +420,46 @@ __global__ __launch_bounds__(256) void rec_rows_kernel(const RecArgs a)
         Map<S> m[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) m[v] = {S(1), S(0), false};
+        auto reduce = [&](auto edges) {
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int64_t r = row_at(i);
-            if (inside(r)) {
-                if (enters >> i & 1) {
+            for (int i = 0; i < R; ++i) {
+                if (decltype(edges)::value && !(valid >> i & 1)) continue;
+                if (decltype(edges)::value && (enters >> i & 1)) {
 #pragma unroll
                     for (int v = 0; v < V; ++v) {
-                        m[v].H = edge ? edge[seq[i] * edge_r + c + v] : S(0);
+                        // (what stands in front of the last entry does not come through)
+                        m[v].H = edge && live && !(enters >> i >> 1) ? edge[seq[i] * edge_r + c + v] : S(0);
                         m[v].cut = true;
                     }
                 }
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    step(i, v, m[v].H, m[v].H);
-                    m[v].A *= gate_at(i, v).a;
+                    const Gate<S> g = gate_at(i, v);
+                    step(g, widen(raw[i].v[v]), m[v].H);
+                    if (!SHARED || v == 0) m[v].A *= g.a;
                 }
             }
-        }
+        };
+        if (plain)
+            reduce(std::false_type());
+        else
+            reduce(std::true_type());
+        if constexpr (SHARED)
+#pragma unroll
+            for (int v = 1; v < V; ++v) m[v].A = m[0].A;
         // across the stretches of the wave (lanes `across` apart), then across the waves
         Map<S> before[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            for (int d = across; d < 64; d *= 2) {
-                const Map<S> p = shift_up(m[v], d);
-                if (lane >= d) m[v] = join(p, m[v]);
+            before[v] = {S(1), S(0), false};
+            if constexpr (!UNIFORM) {
+                for (int d = across; d < 64; d *= 2) {
+                    const Map<S> p = shift_up(m[v], d);
+                    if (lane >= d) m[v] = join(p, m[v]);
+                }
+                const Map<S> p = shift_up(m[v], across);
+                if (group > 0) before[v] = p;
             }
-            before[v] = shift_up(m[v], across);
-            if (group == 0) before[v] = {S(1), S(0), false};
             if (group == groups - 1) {
                 mapA[wave][v][cl] = m[v].A;
                 mapH[wave][v][cl] = m[v].H;
@@ -383,7 +469,7 @@ __global__ __launch_bounds__(256) void rec_rows_kernel(const RecArgs a)
         __syncthreads();
         for (int v = wave; v < V; v += waves) {
             if (lane < across) {
-                const int64_t ch = ((int64_t)(item % a.blocks) * across + lane) * V + v;
+                const int64_t ch = ((int64_t)(item % (unsigned)a.blocks) * across + lane) * V + v;
                 S st = S(0);
                 if (a.tiles > 1 && ch < a.d) {
                     Map<S> all = {mapA[0][v][lane], mapH[0][v][lane], mapC[0][v][lane] != 0};
@@ -391,25 +477,35 @@ __global__ __launch_bounds__(256) void rec_rows_kernel(const RecArgs a)
                     unsigned long long* words = (unsigned long long*)a.maps;
                     unsigned long long* states = (unsigned long long*)a.carry;
                     publish(words + (pos * a.d + ch) * kMapWords<S>, all);
+                    // the maps of the block first, made one, so that only one product lies between a state's arrival and the next one's leaving
                     const int64_t block = pos / kRowsWindow, from = block * kRowsWindow;
                     const int ahead = (int)(pos - from);
-                    Map<S> seen[kRowsWindow - 1];
-                    for (int poll = 0;; ++poll) {
-                        bool ok = block == 0 || get_state(states + (block - 1) * a.d + ch, st);
+                    Map<S> sum = {S(1), S(0), false};
+                    for (int k0 = 0; k0 < ahead; k0 += 8) {
+                        Map<S> seen[8];
+                        for (int poll = 0;; ++poll) {
+                            bool ok = true;
 #pragma unroll
-                        for (int k = 0; k < kRowsWindow - 1; ++k)
-                            if (k < ahead) ok = published(words + ((from + k) * a.d + ch) * kMapWords<S>, seen[k]) && ok;
-                        if (ok) break;
+                            for (int k = 0; k < 8; ++k) {
+                                const int64_t at = from + (k0 + k < ahead ? k0 + k : k0);
+                                ok = published(words + (at * a.d + ch) * kMapWords<S>, seen[k]) && ok;
+                            }
+                            if (ok || poll == kPolls) break;
+                            __builtin_amdgcn_s_sleep(1);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            if (k0 + k < ahead) sum = join(sum, seen[k]);
+                    }
+                    for (int poll = 0; block > 0; ++poll) {
+                        if (get_state(states + (block - 1) * a.d + ch, st)) break;
                         if (poll == kPolls) {
                             st = S(NAN);
                             break;
                         }
-                        __builtin_amdgcn_s_sleep(1);
                     }
-#pragma unroll
-                    for (int k = 0; k < kRowsWindow - 1; ++k)
-                        if (k < ahead) st = seen[k].of(st);
-                    if (ahead == kRowsWindow - 1) put_state(states + block * a.d + ch, all.of(st));
+                    if (ahead == kRowsWindow - 1) put_state(states + block * a.d + ch, join(sum, all).of(st));
+                    st = sum.of(st);
                 }
                 front[v][lane] = st;
             }
@@ -426,27 +522,52 @@ __global__ __launch_bounds__(256) void rec_rows_kernel(const RecArgs a)
         for (int v = 0; v < V; ++v) state[v] = S(0);
     }
 
+    // the states that the next rows' sequences are entered with: loads under a condition would be waited for one by one
+    S given[BATCH][V];
+    auto fetch = [&](int i0) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int64_t s = enters >> (i0 + i) & 1 ? seq[i0 + i] : 0;
+            if (edge) {
+                const Run<S, V> r = load_run<S, V>(edge + s * edge_r + cc);
+#pragma unroll
+                for (int v = 0; v < V; ++v) given[i][v] = r.v[v];
+            } else
+#pragma unroll
+                for (int v = 0; v < V; ++v) given[i][v] = S(0);
+        }
+    };
+
     // the walk itself
     if constexpr (!BACKWARD) {
-        T* __restrict__ out = (T*)a.h + cc;
+        T* out = (T*)a.h;
         S* last = (S*)a.last;
+        auto walk = [&](auto edges) {
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int64_t r = row_at(i);
-            if (inside(r)) {
-                if (enters >> i & 1) {
+            for (int i = 0; i < R; ++i) {
+                if (decltype(edges)::value && i % BATCH == 0) fetch(i);
+                if (decltype(edges)::value && !(valid >> i & 1)) continue;
+                if (decltype(edges)::value && (enters >> i & 1)) {
 #pragma unroll
-                    for (int v = 0; v < V; ++v) state[v] = edge ? edge[seq[i] * edge_r + c + v] : S(0);
+                    for (int v = 0; v < V; ++v) state[v] = given[i % BATCH][v];
                 }
                 Run<T, V> y;
 #pragma unroll
-                for (int v = 0; v < V; ++v) y.v[v] = narrow<T>(step(i, v, state[v], state[v]));
-                store_run<T, V>(out + r * a.h_r, y);
-                if (last && (leaves >> i & 1)) {
+                for (int v = 0; v < V; ++v) y.v[v] = narrow<T>(step(gate_at(i, v), widen(raw[i].v[v]), state[v]));
+                store_run<T, V>(out + row_at(i) * a.h_r + c, y);
+                if (decltype(edges)::value && last && (leaves >> i & 1)) {
+                    Run<S, V> r;
 #pragma unroll
-                    for (int v = 0; v < V; ++v) last[seq[i] * a.last_r + c + v] = state[v];
+                    for (int v = 0; v < V; ++v) r.v[v] = state[v];
+                    store_run<S, V>(last + seq[i] * a.last_r + c, r);
                 }
             }
+        };
+        if (live) {
+            if (plain)
+                walk(std::false_type());
+            else
+                walk(std::true_type());
         }
         if (last)  // sequences without rows end in the state they began with
             for (int64_t s0 = pos * (waves * groups) + wave * groups + group; s0 < a.nseq; s0 += a.tiles * (waves * groups))
@@ -454,76 +575,86 @@ __global__ __launch_bounds__(256) void rec_rows_kernel(const RecArgs a)
 #pragma unroll
                     for (int v = 0; v < V; ++v) last[s0 * a.last_r + c + v] = edge ? edge[s0 * edge_r + c + v] : S(0);
     } else {
-        const T* __restrict__ hin = (const T*)a.hin + cc;
-        const T* __restrict__ x = (const T*)a.x + cc;
+        const T* hin = (const T*)a.hin;
+        const T* x = (const T*)a.x;
         const S* h0 = (const S*)a.h0;
         S* dh0 = (S*)a.dh0;
-        T* __restrict__ dx = (T*)a.dx + cc;
+        T* dx = (T*)a.dx;
+        auto walk = [&](auto edges) {
 #pragma unroll
-        for (int i0 = 0; i0 < R; i0 += BATCH) {
-            Run<T, V> hb[BATCH], xb[FORM == FR_GATE_STATIONARY ? BATCH : 1];
-            if (a.dgate && a.n > 0) {
+            for (int i0 = 0; i0 < R; i0 += BATCH) {
+                Run<T, V> hb[BATCH], xb[FORM == FR_GATE_STATIONARY ? BATCH : 1];
+                if (a.dgate && a.n > 0) {
+#pragma unroll
+                    for (int i = 0; i < BATCH; ++i) {
+                        hb[i] = load_run<T, V>(hin + address_row(row_at(i0 + i) - 1) * a.h_r + cc);
+                        if constexpr (FORM == FR_GATE_STATIONARY) xb[i] = load_run<T, V>(x + address_row(row_at(i0 + i)) * a.x_r + cc);
+                    }
+                }
+                S sum[BATCH];
+                if (decltype(edges)::value) fetch(i0);
 #pragma unroll
                 for (int i = 0; i < BATCH; ++i) {
-                    hb[i] = load_run<T, V>(hin + address_row(row_at(i0 + i) - 1) * a.h_r);
-                    if constexpr (FORM == FR_GATE_STATIONARY) xb[i] = load_run<T, V>(x + address_row(row_at(i0 + i)) * a.x_r);
-                }
-            }
-            S sum[BATCH];
+                    const int64_t r = row_at(i0 + i);
+                    sum[i] = S(0);
+                    if (decltype(edges)::value && !(valid >> (i0 + i) & 1)) continue;
+                    if (decltype(edges)::value && (enters >> (i0 + i) & 1)) {
 #pragma unroll
-            for (int i = 0; i < BATCH; ++i) {
-                const int64_t r = row_at(i0 + i);
-                sum[i] = S(0);
-                if (inside(r)) {
-                    if (enters >> (i0 + i) & 1) {
-#pragma unroll
-                        for (int v = 0; v < V; ++v) state[v] = edge ? edge[seq[i0 + i] * edge_r + c + v] : S(0);
+                        for (int v = 0; v < V; ++v) state[v] = given[i][v];
                     }
-                    const bool first = leaves >> (i0 + i) & 1;
+                    const bool first = decltype(edges)::value && (leaves >> (i0 + i) & 1);
                     Run<T, V> y, z;
 #pragma unroll
                     for (int v = 0; v < V; ++v) {
-                        const S G = step(i0 + i, v, state[v], state[v]);
                         const Gate<S> g = gate_at(i0 + i, v);
+                        const S G = step(g, widen(raw[i0 + i].v[v]), state[v]);
                         y.v[v] = narrow<T>(FORM == FR_GATE_STATIONARY ? g.c * G : G);
                         if (a.dgate) {
-                            const S prev = !first ? widen(hb[i].v[v]) : (h0 ? h0[seq[i0 + i] * a.h0_r + c + v] : S(0));
+                            S prev = widen(hb[i].v[v]);
+                            if (first) prev = h0 && live ? h0[seq[i0 + i] * a.h0_r + c + v] : S(0);
                             const S dg = gate_grad<FORM, S>(g, G, prev, FORM == FR_GATE_STATIONARY ? widen(xb[FORM == FR_GATE_STATIONARY ? i : 0].v[v]) : S(0));
                             if constexpr (SHARED) {
                                 sum[i] += dg;
-                                if (a.sum_lanes == 0) ((S*)a.part)[r * a.part_r + (c + v) * a.part_c] = dg;
+                                if (a.sum_lanes == 0 && live) ((S*)a.part)[r * a.part_r + (c + v) * a.part_c] = dg;
                             } else
                                 z.v[v] = narrow<T>(dg);
                         }
                     }
-                    if (a.dx) store_run<T, V>(dx + r * a.dx_r, y);
-                    if constexpr (!SHARED)
-                        if (a.dgate) store_run<T, V>((T*)a.dgate + r * a.dg_r + c, z);
-                    if (dh0 && first) {
+                    if (live) {
+                        if (a.dx) store_run<T, V>(dx + r * a.dx_r + c, y);
+                        if constexpr (!SHARED)
+                            if (a.dgate) store_run<T, V>((T*)a.dgate + r * a.dg_r + c, z);
+                        if (dh0 && first) {
 #pragma unroll
-                        for (int v = 0; v < V; ++v) dh0[seq[i0 + i] * a.dh0_r + c + v] = state[v];
-                    }
+                            for (int v = 0; v < V; ++v) dh0[seq[i0 + i] * a.dh0_r + c + v] = state[v];
+                        }
+                    } else
+                        sum[i] = S(0);
                 }
-            }
-            if constexpr (SHARED) {
-                if (a.dgate && a.sum_lanes > 0) {
-                    for (int d = 1; d < a.sum_lanes; d *= 2)
+                if constexpr (SHARED) {
+                    if (a.dgate && a.sum_lanes > 0) {
+                        for (int d = 1; d < a.sum_lanes; d *= 2)
 #pragma unroll
-                        for (int i = 0; i < BATCH; ++i) sum[i] += __shfl_xor(sum[i], d);
-                    if ((cl & (a.sum_lanes - 1)) == 0) {
+                            for (int i = 0; i < BATCH; ++i) sum[i] += __shfl_xor(sum[i], d);
+                        if (live && (cl & (a.sum_lanes - 1)) == 0) {
 #pragma unroll
-                        for (int i = 0; i < BATCH; ++i) {
-                            const int64_t r = row_at(i0 + i);
-                            if (!inside(r)) continue;
-                            if (a.pieces == 1)
-                                ((T*)a.dgate)[r * a.dg_r + c / a.width] = narrow<T>(sum[i]);
-                            else
-                                ((S*)a.part)[r * a.part_r + c / (64 * V)] = sum[i];
+                            for (int i = 0; i < BATCH; ++i) {
+                                const int64_t r = row_at(i0 + i);
+                                if (decltype(edges)::value && !(valid >> (i0 + i) & 1)) continue;
+                                if (a.pieces == 1)
+                                    ((T*)a.dgate)[r * a.dg_r + gc0] = narrow<T>(sum[i]);
+                                else
+                                    ((S*)a.part)[r * a.part_r + c / (64 * V)] = sum[i];
+                            }
                         }
                     }
                 }
             }
-        }
+        };
+        if (plain)
+            walk(std::false_type());
+        else
+            walk(std::true_type());
         if (dh0)
             for (int64_t s0 = pos * (waves * groups) + wave * groups + group; s0 < a.nseq; s0 += a.tiles * (waves * groups))
                 if (live && seq_row(a, s0 + 1) <= seq_row(a, s0))
@@ -538,16 +669,16 @@ __global__ __launch_bounds__(256) void rec_rows_kernel(const RecArgs a)
 // exponential worked out, once for those channels.
 
 template <typename T, int FORM, int CG, bool BACKWARD>
-__global__ __launch_bounds__(256) void rec_columns_kernel(const RecArgs a)
+__global__ __launch_bounds__(512) void rec_columns_kernel(const RecArgs a)
 {
     using S = wide_t<T>;
     constexpr int E = kRowsOfLane;
     __shared__ unsigned slot;
-    __shared__ S mapA[CG][4], mapH[CG][4], front[CG];
-    __shared__ int mapC[CG][4];
-    __shared__ int sequence[256][E + 1];  // of a lane's rows that begin or end one (a stride that spreads the banks)
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const unsigned item = claim_tile(a, &slot);
+    __shared__ S mapA[kWaves], mapH[CG][kWaves], front[CG];
+    __shared__ int mapC[kWaves];
+    __shared__ int sequence[64 * kWaves][E + 1];  // of a lane's rows that begin or end one (a stride that spreads the banks)
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const unsigned item = __builtin_amdgcn_readfirstlane(claim_tile(a, &slot));
     const int64_t pos = item / a.blocks;
     const int64_t block = item % a.blocks, q = block / a.pieces, piece = block % a.pieces;
     const int64_t c0 = q * a.width + piece * CG;
@@ -600,7 +731,20 @@ __global__ __launch_bounds__(256) void rec_columns_kernel(const RecArgs a)
     const S* edge = (const S*)(BACKWARD ? a.dlast : a.h0);
     const int64_t edge_c = BACKWARD ? a.dlast_c : a.h0_c;
     int* seq = sequence[threadIdx.x];
-    if (any) find_edges<E, BACKWARD>(a, row0, rb, re, enters, leaves, seq);
+    bool edges = true;
+    if (a.nseq > 1) {  // most waves lie inside one sequence
+        const int64_t w0 = pos * blockDim.x + wave * 64, w1 = w0 + 64 < a.stretches ? w0 + 64 : a.stretches;
+        const int64_t r0 = BACKWARD ? (a.stretches - w1) * E : w0 * E, r1 = BACKWARD ? (a.stretches - w0) * E : w1 * E;
+        const int64_t b = r0 > lo ? r0 : lo, e = r1 < hi ? r1 : hi;
+        edges = false;
+        if (b < e) {
+            int64_t base;
+            const int64_t first = wave_sequences(a, b, base);
+            bool many;
+            edges = wave_edges(first, b, e, many) || many;
+        }
+    }
+    if (any && edges) find_edges<E, BACKWARD>(a, lo, hi, row0, rb, re, enters, leaves, seq);
     if (enters && edge) {
 #pragma unroll
         for (int i = 0; i < E; ++i)
@@ -626,78 +770,95 @@ __global__ __launch_bounds__(256) void rec_columns_kernel(const RecArgs a)
         }
     };
 
-    S state[CG], wave_a = S(1);
-    bool wave_cut = false;
+    // the map of the lane's rows (the channels share its factor), of the rows of the lanes before it, and of the wave
+    S A = S(1), H[CG];
+    bool cut = enters != 0;
 #pragma unroll
-    for (int j = 0; j < CG; ++j) {
-        state[j] = S(0);
-        if (j >= ng) continue;
-        Map<S> m = {S(1), S(0), enters != 0};
+    for (int j = 0; j < CG; ++j) H[j] = S(0);
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-            if (valid >> i & 1) {
-                step(i, u[j][i], m.H, m.H);
-                m.A *= ga[i];
-            }
-        for (int d = 1; d < 64; d *= 2) {
-            const Map<S> p = shift_up(m, d);
-            if (lane >= d) m = join(p, m);
+    for (int i = 0; i < E; ++i)
+        if (valid >> i & 1) {
+#pragma unroll
+            for (int j = 0; j < CG; ++j) step(i, u[j][i], H[j], H[j]);
+            A *= ga[i];
         }
-        if (lane == 63) {
-            mapA[j][wave] = m.A;
-            mapH[j][wave] = m.H;
-            mapC[j][wave] = m.cut;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const S pa = __shfl_up(A, d);
+        const bool pc = __shfl_up((int)cut, d);
+#pragma unroll
+        for (int j = 0; j < CG; ++j) {
+            const S ph = __shfl_up(H[j], d);
+            if (lane >= d && !cut) H[j] = A * ph + H[j];
         }
-        Map<S> before = shift_up(m, 1);
-        if (lane == 0) before = {S(1), S(0), false};
-        // (kept in the place of the state until the workgroup's is known)
-        state[j] = before.H;
-        if (j == 0) {
-            wave_a = before.A;
-            wave_cut = before.cut;
+        if (lane >= d) {
+            A *= pa;
+            cut = cut || pc;
         }
+    }
+    if (lane == 63) {
+        mapA[wave] = A;
+        mapC[wave] = cut;
+#pragma unroll
+        for (int j = 0; j < CG; ++j) mapH[j][wave] = H[j];
+    }
+    A = __shfl_up(A, 1);
+    cut = __shfl_up((int)cut, 1);
+#pragma unroll
+    for (int j = 0; j < CG; ++j) H[j] = __shfl_up(H[j], 1);
+    if (lane == 0) {
+        A = S(1), cut = false;
+#pragma unroll
+        for (int j = 0; j < CG; ++j) H[j] = S(0);
     }
     __syncthreads();
     for (int j = wave; j < ng; j += waves) {
         S st = S(0);
         if (a.tiles > 1) {
-            Map<S> all = {mapA[j][0], mapH[j][0], mapC[j][0] != 0};
-            for (int k = 1; k < waves; ++k) all = join(all, Map<S>{mapA[j][k], mapH[j][k], mapC[j][k] != 0});
-            unsigned long long* words = (unsigned long long*)a.maps;
-            unsigned long long* states = (unsigned long long*)a.carry;
-            const int64_t ch = c0 + j;
-            if (lane == 0) publish(words + (pos * a.d + ch) * kMapWords<S>, all);
-            const int64_t window = pos / 64, from = window * 64;
+            Map<S> all = {mapA[0], mapH[j][0], mapC[0] != 0};
+            for (int k = 1; k < waves; ++k) all = join(all, Map<S>{mapA[k], mapH[j][k], mapC[k] != 0});
+            // (a channel's words lie side by side: a wave reads the window's in a few lines)
+            unsigned long long* words = (unsigned long long*)a.maps + (c0 + j) * a.tiles * kMapWords<S>;
+            unsigned long long* states = (unsigned long long*)a.carry + (c0 + j) * (a.tiles / kColumnsWindow + 1);
+            if (lane == 0) publish(words + pos * kMapWords<S>, all);
+            // the maps of the window first, made one, so that only one product lies between a state's arrival and the next one's leaving
+            const int64_t window = pos / kColumnsWindow, from = window * kColumnsWindow;
             const int ahead = (int)(pos - from);
             Map<S> m = {S(1), S(0), false};
             for (int poll = 0;; ++poll) {
-                bool ok = window == 0 || get_state(states + (window - 1) * a.d + ch, st);
-                if (lane < ahead) ok = published(words + ((from + lane) * a.d + ch) * kMapWords<S>, m) && ok;
-                if (__all(ok)) break;
+                const bool ok = lane >= ahead || published(words + (from + lane) * kMapWords<S>, m);
+                if (__all(ok) || poll == kPolls) break;
+                __builtin_amdgcn_s_sleep(2);
+            }
+            if (lane >= ahead) m = {S(1), S(0), false};
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+                const Map<S> p = shift_up(m, d);
+                if (lane >= d) m = join(p, m);
+            }
+            m = {__shfl(m.A, 63), __shfl(m.H, 63), (bool)__shfl((int)m.cut, 63)};
+            const Map<S> through = join(m, all);
+            for (int poll = 0; window > 0; ++poll) {
+                if (get_state(states + window - 1, st)) break;
                 if (poll == kPolls) {
                     st = S(NAN);
                     break;
                 }
                 __builtin_amdgcn_s_sleep(1);
             }
-            if (lane >= ahead) m = {S(1), S(0), false};
-            for (int d = 1; d < 64; d *= 2) {
-                const Map<S> p = shift_up(m, d);
-                if (lane >= d) m = join(p, m);
-            }
-            m = {__shfl(m.A, 63), __shfl(m.H, 63), (bool)__shfl((int)m.cut, 63)};
+            if (ahead == kColumnsWindow - 1 && lane == 0) put_state(states + window, through.of(st));
             st = m.of(st);
-            if (ahead == 63 && lane == 0) put_state(states + window * a.d + ch, all.of(st));
         }
         if (lane == 0) front[j] = st;
     }
     __syncthreads();
+    S state[CG];
 #pragma unroll
     for (int j = 0; j < CG; ++j) {
         if (j >= ng) continue;
         S st = front[j];
-        for (int k = 0; k < wave; ++k) st = Map<S>{mapA[j][k], mapH[j][k], mapC[j][k] != 0}.of(st);
-        state[j] = Map<S>{wave_a, state[j], wave_cut}.of(st);
+        for (int k = 0; k < wave; ++k) st = Map<S>{mapA[k], mapH[j][k], mapC[k] != 0}.of(st);
+        state[j] = cut ? H[j] : A * st + H[j];
     }
 
     if constexpr (!BACKWARD) {
@@ -813,12 +974,12 @@ __global__ __launch_bounds__(256) void rec_heads_kernel(const RecArgs a)
 
 // The workgroups along the rows, and the memory that passes states between them (none for a single one)
 template <typename T>
-static int rec_prepare(fr_ctx* ctx, RecArgs& a, int64_t rows, int64_t stretches_of_wave, int64_t window, int64_t parts, OpWorkspace& ws, int* waves)
+static int rec_prepare(fr_ctx* ctx, RecArgs& a, int64_t rows, int64_t stretches_of_wave, int most, int64_t window, int64_t parts, OpWorkspace& ws, int* waves)
 {
     using S = wide_t<T>;
     a.stretches = (a.n + rows - 1) / rows;
     int64_t w = (a.stretches + stretches_of_wave - 1) / stretches_of_wave;
-    *waves = (int)(w < 1 ? 1 : (w > 4 ? 4 : w));
+    *waves = (int)(w < 1 ? 1 : (w > most ? most : w));
     a.tiles = (a.stretches + *waves * stretches_of_wave - 1) / (*waves * stretches_of_wave);
     if (a.tiles < 1) a.tiles = 1;
     if (a.tiles * a.blocks > 0x7fffffffLL / 256 * 64) return set_err(ctx, FR_SHAPE, "%lld rows of %lld channels are too many for one call", (long long)a.n, (long long)a.d);
@@ -859,12 +1020,23 @@ static int rec_rows(fr_ctx* ctx, RecArgs& a, bool backward, OpWorkspace& ws)
         }
     }
     int waves;
-    FR_TRY(rec_prepare<T>(ctx, a, kRowsOf<T, SHARED>, 64 / across, kRowsWindow, parts, ws, &waves));
+    const bool few = !backward && a.lanes == 6 && a.n <= kFewRows;
+    const int64_t rows = few ? kRowsOf<T, FORM, SHARED, true, false, true> : backward || a.lanes < 6 ? kRowsOf<T, FORM, SHARED, true, true, false> : kRowsOf<T, FORM, SHARED, true, false, false>;
+    FR_TRY(rec_prepare<T>(ctx, a, rows, 64 / across, kWaves, kRowsWindow, parts, ws, &waves));
     const dim3 grid((unsigned)(a.tiles * a.blocks)), block(64 * waves);
-    if (backward)
-        hipLaunchKernelGGL((rec_rows_kernel<T, FORM, V, SHARED, true>), grid, block, 0, ctx->ls, a);
-    else
-        hipLaunchKernelGGL((rec_rows_kernel<T, FORM, V, SHARED, false>), grid, block, 0, ctx->ls, a);
+    auto launch = [&](auto uniform) {
+        constexpr bool U = decltype(uniform)::value;
+        if (backward)
+            hipLaunchKernelGGL((rec_rows_kernel<T, FORM, V, SHARED, true, U, false>), grid, block, 0, ctx->ls, a);
+        else
+            hipLaunchKernelGGL((rec_rows_kernel<T, FORM, V, SHARED, false, U, false>), grid, block, 0, ctx->ls, a);
+    };
+    if (few)
+        hipLaunchKernelGGL((rec_rows_kernel<T, FORM, V, SHARED, false, true, true>), grid, block, 0, ctx->ls, a);
+    else if (V > 1 || a.lanes == 6)
+        launch(std::true_type());
+    else if constexpr (V == 1)
+        launch(std::false_type());
     return FR_OK;
 }
 
@@ -876,7 +1048,7 @@ static int rec_columns(fr_ctx* ctx, RecArgs& a, bool backward, OpWorkspace& ws)
     const bool join = backward && a.dgate && a.pieces > 1;
     a.part_r = 1, a.part_c = a.n;
     int waves;
-    FR_TRY(rec_prepare<T>(ctx, a, kRowsOfLane, 64, 64, join ? a.blocks * a.n : 0, ws, &waves));
+    FR_TRY(rec_prepare<T>(ctx, a, kRowsOfLane, 64, kWaves, kColumnsWindow, join ? a.blocks * a.n : 0, ws, &waves));
     const dim3 grid((unsigned)(a.tiles * a.blocks)), block(64 * waves);
     if (backward)
         hipLaunchKernelGGL((rec_columns_kernel<T, FORM, CG, true>), grid, block, 0, ctx->ls, a);

@@ -45,9 +45,7 @@ __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half(
 template <>
 __device__ __forceinline__ __hip_bfloat16 narrow<__hip_bfloat16>(float v)
 {
-    const unsigned u = __float_as_uint(v);
-    // (a NaN keeps its top bits and a quiet bit; adding the rounding term could carry it into infinity)
-    const unsigned short b = v != v ? (unsigned short)((u >> 16) | 0x40u) : (unsigned short)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+    const __bf16 b = (__bf16)v;  // (v_cvt_pk_bf16_f32)
     __hip_bfloat16 r;
     __builtin_memcpy(&r, &b, 2);
     return r;
