@@ -64,16 +64,28 @@ __global__ __launch_bounds__(kPlanThreads) void experts_plan_kernel(const PlanAr
     const int m = (int)a.m, k = (int)a.k;
     const int share = (m + WAVES * 64 - 1) / (WAVES * 64) * 64;
     const int lo = wave * share < m ? wave * share : m, hi = lo + share < m ? lo + share : m;
-    int own = 0, early = 0;
-    for (int j = 0; j < k; ++j) {
+    // eight looks at a time: the stores of the second walk would put each load behind the one before it
+    constexpr int LOOKS = 8;
+    auto look = [&](int j, int q, int (&at)[LOOKS]) {
         const int* chosen = a.chosen + j * a.lde;
-#pragma unroll 4
-        for (int q = lo; q < hi; q += 64) {
-            const int v = chosen[q + lane < hi ? q + lane : hi - 1], at = q + lane < hi ? v : -1;
-            own += __popcll(__ballot(at == e));
-            early += __popcll(__ballot(at >= 0 && at < e));
+#pragma unroll
+        for (int i = 0; i < LOOKS; ++i) {
+            const int p = q + 64 * i + lane;
+            const int v = chosen[p < hi ? p : hi - 1];
+            at[i] = p < hi ? v : -1;
         }
-    }
+    };
+    int own = 0, early = 0;
+    for (int j = 0; j < k; ++j)
+        for (int q = lo; q < hi; q += 64 * LOOKS) {
+            int at[LOOKS];
+            look(j, q, at);
+#pragma unroll
+            for (int i = 0; i < LOOKS; ++i) {
+                own += __popcll(__ballot(at[i] == e));
+                early += __popcll(__ballot(at[i] >= 0 && at[i] < e));
+            }
+        }
     if (lane == 0) {
         mine[wave] = own;
         before[wave] = early;
@@ -90,21 +102,23 @@ __global__ __launch_bounds__(kPlanThreads) void experts_plan_kernel(const PlanAr
         a.starts[e] = start;
         if (e == a.experts - 1) a.starts[a.experts] = start + total;
     }
-    for (int j = 0; j < k; ++j) {
-        const int* chosen = a.chosen + j * a.lde;
-#pragma unroll 4
-        for (int q = lo; q < hi; q += 64) {
-            const int v = chosen[q + lane < hi ? q + lane : hi - 1], at = q + lane < hi ? v : -1;
-            const unsigned long long all = __ballot(at == e);
-            if (at == e) {
-                const int p = place + __popcll(all & ((1ull << lane) - 1));
-                a.place[j * a.m + q + lane] = p;
-                a.list[p] = (int)(j * a.m) + q + lane;
-            } else if (e == 0 && q + lane < hi && (at < 0 || at >= a.experts))
-                a.place[j * a.m + q + lane] = -1;
-            place += __popcll(all);
+    for (int j = 0; j < k; ++j)
+        for (int q = lo; q < hi; q += 64 * LOOKS) {
+            int at[LOOKS];
+            look(j, q, at);
+#pragma unroll
+            for (int i = 0; i < LOOKS; ++i) {
+                const unsigned long long all = __ballot(at[i] == e);
+                const int slot = q + 64 * i + lane;
+                if (at[i] == e) {
+                    const int p = place + __popcll(all & ((1ull << lane) - 1));
+                    a.place[j * a.m + slot] = p;
+                    a.list[p] = (int)(j * a.m) + slot;
+                } else if (e == 0 && slot < hi && (at[i] < 0 || at[i] >= a.experts))
+                    a.place[j * a.m + slot] = -1;
+                place += __popcll(all);
+            }
         }
-    }
     __syncthreads();  // (the list is this workgroup's own: no other reads or writes its part)
     for (int i = threadIdx.x; i < total; i += kPlanThreads) {
         const int slot = a.list[start + i], j = slot / m, q = slot - j * m;
@@ -471,7 +485,9 @@ static void leaf_launch(fr_ctx* ctx, const BlockArgs& a, dim3 grid)
         hipLaunchKernelGGL((experts_lanes_kernel<LEAF, 1>), grid, block, 0, ctx->ls, a);
     else if (a.d <= 8)
         hipLaunchKernelGGL((experts_lanes_kernel<LEAF, 2>), grid, block, 0, ctx->ls, a);
-    else if (a.d <= 16 && a.d > 12)
+    else if (a.d <= 12)
+        hipLaunchKernelGGL((experts_lanes_kernel<LEAF, 3>), grid, block, 0, ctx->ls, a);
+    else if (a.d <= 16)
         hipLaunchKernelGGL((experts_lanes_kernel<LEAF, 4>), grid, block, 0, ctx->ls, a);
     else
         hipLaunchKernelGGL((experts_lanes_kernel<LEAF, 0>), grid, block, 0, ctx->ls, a);
@@ -549,7 +565,7 @@ int fr_experts_predict(fr_ctx* ctx, const fr_kprog* kernel, const double* X, int
         if (out_slots) FR_TRY(os.stage(out_slots, m, k, lds, 8, "out_slots", true));
         if (m == 0) return FR_OK;
         const int64_t slots = m * k;
-        // few: [MEASURED]
+        // few slots an expert: sums over lanes of points; many: a lane for each slot (both sides measured: see experts_few_kernel)
         const bool few = slots < n_experts * 64;
         const int64_t used = slots < n_experts ? slots : n_experts, blocks = (slots + 7) / 8 + used, tiles = few ? blocks : slots / kSide + used;
         const int64_t want = (int64_t)ctx->num_cus * (few ? 4 : 20);

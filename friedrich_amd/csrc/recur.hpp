@@ -481,6 +481,7 @@ __global__ __launch_bounds__(512) void rec_rows_kernel(const RecArgs a)
                     const int64_t block = pos / kRowsWindow, from = block * kRowsWindow;
                     const int ahead = (int)(pos - from);
                     Map<S> sum = {S(1), S(0), false};
+                    bool lost = false;
                     for (int k0 = 0; k0 < ahead; k0 += 8) {
                         Map<S> seen[8];
                         for (int poll = 0;; ++poll) {
@@ -490,13 +491,15 @@ __global__ __launch_bounds__(512) void rec_rows_kernel(const RecArgs a)
                                 const int64_t at = from + (k0 + k < ahead ? k0 + k : k0);
                                 ok = published(words + (at * a.d + ch) * kMapWords<S>, seen[k]) && ok;
                             }
-                            if (ok || poll == kPolls) break;
+                            lost |= poll == kPolls;
+                            if (ok || lost) break;
                             __builtin_amdgcn_s_sleep(1);
                         }
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
                             if (k0 + k < ahead) sum = join(sum, seen[k]);
                     }
+                    if (lost) sum = {S(1), S(NAN), true};
                     for (int poll = 0; block > 0; ++poll) {
                         if (get_state(states + (block - 1) * a.d + ch, st)) break;
                         if (poll == kPolls) {
@@ -825,12 +828,15 @@ __global__ __launch_bounds__(512) void rec_columns_kernel(const RecArgs a)
             const int64_t window = pos / kColumnsWindow, from = window * kColumnsWindow;
             const int ahead = (int)(pos - from);
             Map<S> m = {S(1), S(0), false};
+            bool lost = false;
             for (int poll = 0;; ++poll) {
                 const bool ok = lane >= ahead || published(words + (from + lane) * kMapWords<S>, m);
-                if (__all(ok) || poll == kPolls) break;
+                lost = poll == kPolls;
+                if (__all(ok) || lost) break;
                 __builtin_amdgcn_s_sleep(2);
             }
             if (lane >= ahead) m = {S(1), S(0), false};
+            if (lost) m = {S(1), S(NAN), true};
 #pragma unroll
             for (int d = 1; d < 64; d *= 2) {
                 const Map<S> p = shift_up(m, d);
@@ -982,7 +988,7 @@ static int rec_prepare(fr_ctx* ctx, RecArgs& a, int64_t rows, int64_t stretches_
     *waves = (int)(w < 1 ? 1 : (w > most ? most : w));
     a.tiles = (a.stretches + *waves * stretches_of_wave - 1) / (*waves * stretches_of_wave);
     if (a.tiles < 1) a.tiles = 1;
-    if (a.tiles * a.blocks > 0x7fffffffLL / 256 * 64) return set_err(ctx, FR_SHAPE, "%lld rows of %lld channels are too many for one call", (long long)a.n, (long long)a.d);
+    if (a.tiles * a.blocks * 64 * *waves > 0xffffffffLL) return set_err(ctx, FR_SHAPE, "%lld rows of %lld channels are too many for one call", (long long)a.n, (long long)a.d);
     const int64_t maps = a.tiles * a.d * kMapWords<S>, states = (a.tiles / window + 1) * a.d;
     const int64_t words = a.tiles > 1 ? 1 + maps + states : 0;
     if (words + parts == 0) return FR_OK;

@@ -424,6 +424,10 @@ __global__ __launch_bounds__(256, 2) void route_lists_kernel(const RouteArgs a)
             top = v > top ? v : top;
             key[c] = (float)v;
         }
+        bool odd = wild;
+        if constexpr (sizeof(T) == 8)  // (what 32 bits would turn into a closed expert)
+#pragma unroll
+            for (int c = 0; c < C; ++c) odd |= key[c] == -INFINITY && raw[c] != -INFINITY;
         double inverse = 1.0;
         float about = 1.0f;  // 1 / the sum of exponentials in 32 bits
         if constexpr (!SIGMOID) {
@@ -445,7 +449,6 @@ __global__ __launch_bounds__(256, 2) void route_lists_kernel(const RouteArgs a)
             }
         }
         bad = at.lane_any(bad);
-        bool odd = wild;
         if (scored) {
             float rank[C], best = -INFINITY, second = -INFINITY;
 #pragma unroll

@@ -31,6 +31,7 @@ class DeviceMatrix:
 
     def __init__(self, ctx, ptr, rows, cols, ld):
         self.ctx, self.ptr, self.rows, self.cols, self.ld = ctx, ptr, rows, cols, ld
+        self.shape, self.dtype, self.itemsize, self.strides = (rows, cols), np.dtype(np.float64), 8, (8, 8 * ld)  # (read like an array's)
 
     def free(self):
         if self.ptr and getattr(self.ctx, "h", None):
@@ -128,6 +129,8 @@ def _strides(t):
 
 
 def _address(t):
+    if isinstance(t, DeviceMatrix):
+        return t.ptr
     return t.data_ptr() if _is_torch(t) else t.ctypes.data
 
 
@@ -433,6 +436,8 @@ class Context:
                                              ctypes.byref(h)))
         return Cholesky(self, h)
 
+    # (the calls from here on take torch tensors and numpy arrays.  With torch tensors set_stream the stream that torch works on first: the
+    # context's own stream does not wait for it.)
     # ordered inputs: the gated linear recurrence -------------------------------------------------------
     def recurrence(self, gate, x, form="log", offsets=None, h0=None, out=None, last=None):
         """h_t = a_t h_{t-1} + c_t x_t over packed sequences (fr_recurrence).  gate: n x gate_cols, x: n x d, torch tensors or numpy arrays

@@ -359,7 +359,8 @@ int fr_grad_terms(fr_chol* chol, const fr_kprog* kernel, const double* y, double
  *  - device pointers have to belong to the context's device; elements are naturally aligned, nothing more is asked of an address.
  *  - on device data the calls do not wait and may be captured into a HIP graph (fr_ctx_set_stream with the stream that captures).
  *    A capture keeps its workspace until the context is destroyed, and takes it from what eager calls left in the context's pool:
- *    run the calls once before each capture (FR_OUT_OF_MEMORY otherwise).  Host data in a captured call is refused.
+ *    run the calls once before each capture (FR_OUT_OF_MEMORY otherwise).  Host data in a captured call is refused.  Graphs of one
+ *    context may be replayed side by side, one graph not beside itself.
  *  - an output must not overlap an input or another output, except where a call says so. */
 typedef enum { FR_F64 = 0, FR_F32 = 1, FR_BF16 = 2, FR_F16 = 3 } fr_dtype;
 

@@ -60,6 +60,8 @@ def test_route_many_rows(tctx):  # noqa: F811
         z[5::7] = np.round(z[5::7])  # ties
         z[rng.random((n, experts)) < 0.02] = -np.inf
         z[11], z[12, 3] = -np.inf, np.nan
+        if dtype == "f64":  # the type's lowest values are values: only -inf closes
+            z[13], z[14, ::2], z[15, 1:] = np.finfo(np.float64).min, -1e300, -1e39
         flat = np.zeros(experts)
         close = 0.25 + 2.0**-40 * rng.integers(0, 4, experts)
         for bias in (None, flat, close, 0.1 * rng.standard_normal(experts)):
@@ -209,7 +211,7 @@ def model(rng, n, d, experts, m, k, sizes=None, unused=0.0):
 SPECS = [("squared_exp", 0.8, 1.3), ("exponential", 0.9, 0.7), ("matern1", 1.1, 0.9), ("matern2", 0.9, 1.2), ("rational_quadratic", 1.5, 0.8), ("linear", 0.7),
          ("sum", ("prod", ("squared_exp", 1.0, 1.0), ("matern1", 2.0, 0.5)), ("linear", 0.2))]
 # points, features, experts, queries, slots, share of unused slots
-MODELS = [(1, 1, 1, 1, 1, 0.0), (5, 2, 3, 4, 2, 0.0), (64, 3, 1, 64, 1, 0.0), (300, 5, 7, 65, 3, 0.3), (1000, 16, 8, 130, 2, 0.0), (513, 1, 2, 1, 2, 0.0), (2000, 8, 1000, 40, 4, 0.1),
+MODELS = [(300, 11, 2, 400, 1, 0.0), (500, 20, 2, 300, 2, 0.1), (1, 1, 1, 1, 1, 0.0), (5, 2, 3, 4, 2, 0.0), (64, 3, 1, 64, 1, 0.0), (300, 5, 7, 65, 3, 0.3), (1000, 16, 8, 130, 2, 0.0), (513, 1, 2, 1, 2, 0.0), (2000, 8, 1000, 40, 4, 0.1),
           (700, 33, 3, 7, 1, 0.0), (4097, 4, 2, 257, 2, 0.5)]
 
 
@@ -302,6 +304,18 @@ def test_route_to_experts_and_back(tctx):  # noqa: F811
         up[i] += 1e-3
         down[i] -= 1e-3
         assert abs((loss(z, up) - loss(z, down)) / 2e-3 - float(da[i])) <= 1e-8 * (1 + abs(float(da[i])))
+
+
+def test_staged_inputs(tctx):  # noqa: F811
+    """matrices that Context.inputs_to_device has put on the device are taken like arrays"""
+    rng = np.random.default_rng(31)
+    spec = ("matern1", 1.1, 0.9)
+    X, Xq, offsets, chosen, w, alpha = model(rng, 200, 5, 3, 30, 2)
+    x, q = tctx.inputs_to_device(np.ascontiguousarray(X)), tctx.inputs_to_device(Xq, "colmajor")
+    got, slots = tctx.experts_predict(spec, x, alpha, offsets, q, chosen, w)
+    want, _ = tctx.experts_predict(spec, X, alpha, offsets, Xq, chosen, w)
+    assert np.array_equal(got, want)
+    x.free(), q.free()
 
 
 def test_experts_odd_offsets_and_names(tctx):  # noqa: F811

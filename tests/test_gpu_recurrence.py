@@ -91,6 +91,7 @@ def test_one_sequence(tctx, form, dtype, layout):
 
 
 RAGGED = [
+    list(range(0, 300)), [0] * 90 + [1] * 80 + list(range(2, 140)), list(range(0, 1500, 3)) + [4000],
     [0, 1], [0, 1, 2, 3, 4], [0, 0, 5, 5, 5, 9], [3, 3, 40, 41, 41, 100], [0, 700, 1400], [0, 64, 128, 128, 129, 193], [0, 2049, 2050, 4097], [5, 5], [0, 0, 0, 0],
     [0, 16, 32, 48, 64], [0, 511, 1536, 3000],
 ]
@@ -372,6 +373,48 @@ def test_on_another_stream_and_in_a_captured_graph():
     torch.cuda.synchronize()
     del graphs, g
     c.close()
+
+
+def test_two_contexts_at_once():
+    """calls of two threads, each with a context and a stream of its own, in which tiles wait for one another"""
+    import threading
+
+    import torch
+    from friedrich_amd.device import Context
+
+    rng = np.random.default_rng(15)
+    work, errors = [], []
+    for dtype, layout, n, d in (("f64", "col", 600000, 2), ("bf16", "row", 20000, 300)):
+        gate, x, h0, wide = problem(rng, n, d, d, 1, "log", dtype, layout)
+        work.append((gate, x, h0, put(rng.standard_normal((n, d)), layout, x.dtype)))
+    torch.cuda.synchronize()
+
+    def run(gate, x, h0, dh, results):
+        try:
+            c, s = Context(), torch.cuda.Stream()
+            c.set_stream(s.cuda_stream)
+            with torch.cuda.stream(s):
+                for _ in range(6):
+                    h, last = c.recurrence(gate, x, h0=h0)
+                    results.append((h, last) + tuple(c.recurrence_backward(gate, x, h, dh, h0=h0)))
+                s.synchronize()
+            c.close()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    alone, together = [[], []], [[], []]
+    for w, r in zip(work, alone):
+        run(*w, r)
+    threads = [threading.Thread(target=run, args=(*w, r)) for w, r in zip(work, together)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for a, b in zip(alone, together):
+        assert len(b) == 6
+        for r in b:
+            assert all(torch.equal(p, q) for p, q in zip(a[0], r))
 
 
 def test_the_same_call_gives_the_same_bits(tctx):
