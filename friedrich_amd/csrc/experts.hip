@@ -417,29 +417,44 @@ struct JoinArgs {
 __device__ __forceinline__ double add_pieces(const double* part, int64_t ld, int64_t pieces)
 {
     double v = 0.0;
-#pragma unroll 4
-    for (int64_t c = 0; c < pieces; ++c) v += part[c * ld];
+    for (int64_t c0 = 0; c0 < pieces; c0 += 8) {
+        double next[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) next[c] = part[(c0 + c < pieces ? c0 + c : c0) * ld];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v += c0 + c < pieces ? next[c] : 0.0;
+    }
     return v;
 }
 
-// forward: a thread per query point adds up its slots' pieces
-__global__ __launch_bounds__(64) void experts_mean_kernel(const JoinArgs a)
+// Forward: a workgroup takes 64 query points, a thread adds up the pieces of a slot, then the first 64 threads the slots of a point.
+constexpr int kMeanPoints = 64, kMeanThreads = 256;
+__global__ __launch_bounds__(kMeanThreads) void experts_mean_kernel(const JoinArgs a)
 {
-    const int64_t q = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (q >= a.m) return;
-    double mean = a.prior ? a.prior[q] : 0.0;
-    for (int64_t j = 0; j < a.k; ++j) {
+    __shared__ double terms[64][kMeanPoints];
+    const int64_t q0 = (int64_t)blockIdx.x * kMeanPoints;
+    const int points = a.m - q0 < kMeanPoints ? (int)(a.m - q0) : kMeanPoints;
+    for (int i = threadIdx.x; i < (int)a.k * kMeanPoints; i += kMeanThreads) {
+        const int j = i / kMeanPoints, at = i % kMeanPoints;
+        if (at >= points) continue;
+        const int64_t q = q0 + at;
         const int e = a.chosen[q + j * a.lde];
         const int64_t p = a.place[j * a.m + q];
+        const double w = a.weights[q + j * a.ldw];
         double v = 0.0;
         if (p >= 0) {
             const int64_t r0 = row_of(a.begin, e, a.n), r1 = row_of(a.begin, e + 1, a.n);
             v = add_pieces(a.part + p, a.slots, a.few ? (r1 - r0 + a.piece - 1) / a.piece : pieces_of(r0, r1, a.piece));
         }
         if (a.slots_out) a.slots_out[q + j * a.lds] = v;
-        mean += a.weights[q + j * a.ldw] * v;
+        terms[j][at] = w * v;
     }
-    a.mean[q] = mean;
+    __syncthreads();
+    if ((int)threadIdx.x < points) {
+        double mean = a.prior ? a.prior[q0 + threadIdx.x] : 0.0;
+        for (int64_t j = 0; j < a.k; ++j) mean += terms[j][threadIdx.x];
+        a.mean[q0 + threadIdx.x] = mean;
+    }
 }
 
 // backward: the gradient of each coefficient from its pieces, of each weight from its slot's mean
@@ -601,7 +616,7 @@ int fr_experts_predict(fr_ctx* ctx, const fr_kprog* kernel, const double* X, int
         j.m = m, j.k = k, j.slots = slots, j.n = n, j.lde = oe.ld, j.ldw = ow.ld, j.lds = os.ld, j.piece = piece, j.experts = (int)n_experts, j.few = few;
         j.chosen = p.chosen, j.place = p.place, j.begin = oo.as<int64_t>(), j.part = part, j.weights = p.weights, j.prior = op.as<double>();
         j.mean = om.as<double>(), j.slots_out = os.as<double>();
-        hipLaunchKernelGGL(experts_mean_kernel, dim3((unsigned)((m + 63) / 64)), dim3(64), 0, ctx->ls, j);
+        hipLaunchKernelGGL(experts_mean_kernel, dim3((unsigned)((m + kMeanPoints - 1) / kMeanPoints)), dim3(kMeanThreads), 0, ctx->ls, j);
         FR_HIP(ctx, hipGetLastError());
         FR_TRY(om.commit());
         return os.commit();

@@ -677,7 +677,11 @@ template <typename T, int C, bool SIGMOID>
 static void lists_launch(fr_ctx* ctx, const RouteArgs& a, bool backward, dim3 grid)
 {
     const dim3 block(256);
-    if (backward && a.k <= 8)
+    if (backward && a.k <= 2)
+        hipLaunchKernelGGL((route_backward_kernel<T, C, 2, SIGMOID>), grid, block, 0, ctx->ls, a);
+    else if (backward && a.k <= 4)
+        hipLaunchKernelGGL((route_backward_kernel<T, C, 4, SIGMOID>), grid, block, 0, ctx->ls, a);
+    else if (backward && a.k <= 8)
         hipLaunchKernelGGL((route_backward_kernel<T, C, 8, SIGMOID>), grid, block, 0, ctx->ls, a);
     else if (backward)
         hipLaunchKernelGGL((route_backward_kernel<T, C, 0, SIGMOID>), grid, block, 0, ctx->ls, a);
