@@ -38,7 +38,9 @@ __device__ __forceinline__ int64_t block_index(int64_t row, int64_t f, int64_t d
 // A workgroup per expert: every wave counts, among its share of the queries, the slots that name this expert and those that name an earlier
 // one, which is where the expert's list begins; a second walk puts each slot in its place, and the workgroup packs its list's query
 // points.  No atomics: a list's order is that of (share, j, q) on every run.  Every workgroup reads all slots (16384 slots: 64 KB, from
-// L2), which costs less than a launch to sort them first.
+// L2), which costs less than a launch to sort them first.  Bound by
+// latency, the two walks and the packing behind them: 7 us for 6 slots of 16 experts, 15 us for 16384 slots of 64 experts and 65536 points of 16
+// features (8 MB read and written).
 // (loads under a condition are waited for one by one: out of range they read the last place instead)
 __global__ __launch_bounds__(kPlanThreads) void experts_plan_kernel(const PlanArgs a)
 {
@@ -209,8 +211,8 @@ __device__ __forceinline__ double pair_inverse(const fr_kprog& p)
 // Gram kernel does: |x|^2 + |y|^2 - 2 x.y on the matrix cores would lose near points' distances to cancellation, which the square root in
 // three of the kernels turns into an error of 1e-8.  That makes 2 d + about 28 f64 instructions a pair, at 4 cycles a wave and SIMD.  The
 // block comes through scalar loads of one line each, eight points of a feature: it costs no vector register and no LDS traffic (a broadcast
-// read of LDS for every 16 instructions would keep the LDS pipe of the CU busier than its SIMDs), and a block is contiguous: with
-// the features 512 KB apart every load missed the address translation as well, and the kernel waited 70 % of its time.
+// read of LDS for every 16 instructions would keep the LDS pipe of the CU busier than its SIMDs), and a block is contiguous, so its
+// lines need one address.
 template <int LEAF>
 struct Pairs {
     static constexpr bool S = LEAF < 0 || !(LEAF == FR_K_LINEAR || LEAF == FR_K_POLYNOMIAL || LEAF == FR_K_HYPERTAN);
@@ -293,7 +295,10 @@ __device__ __forceinline__ int expert_of(const BlockArgs& a, const int64_t* item
 }
 
 // A lane for each row of the columns' side, the sum over the blocks: an item is a wave of 64 lanes times a piece of blocks.  FOURS > 0: the
-// lanes' features stay in registers; 0: there are more than 16, and they are read again for every block.
+// lanes' features stay in registers; 0: there are more than 16, and they are read again for every block.  Bound by issue of f64
+// instructions: 16777216 pairs of 16 features (squared exponential, 64 experts of 500 to 1500 points) take
+// 61 us, where 60 instructions a pair would take 26; 7500000 in the backward pass 33 us.  20 items a CU even skewed experts out: whole
+// calls with 5, 10, 20 and 32 took 114, 86, 77 and 75 us, backward 49, 45, 44 and 45.
 template <int LEAF, int FOURS>
 __global__ __launch_bounds__(256) void experts_lanes_kernel(const BlockArgs a)
 {
@@ -350,7 +355,10 @@ __global__ __launch_bounds__(256) void experts_lanes_kernel(const BlockArgs a)
 }
 
 // A lane for each row of the columns' side too, but the sum is over the lanes: an item is a block of 8 slots times a piece of the expert's
-// points, which the four waves share out.  For few slots an expert, where lanes of slots would be empty.
+// points, which the four waves share out; the points' features are read again for every block.  For few slots an expert, where lanes of slots
+// would be empty, and for many features (16 experts of 1024 points of 16
+// features, 3 queries of 2 slots: 7 us, most of it latency; 16777216 pairs of 40 features: 102 us, issue).  4 items a CU: with 2, 512 queries
+// of 40 features took 33 us instead of 29, 8 took as long.
 template <int LEAF>
 __global__ __launch_bounds__(256) void experts_few_kernel(const BlockArgs a)
 {
@@ -427,7 +435,8 @@ __device__ __forceinline__ double add_pieces(const double* part, int64_t ld, int
     return v;
 }
 
-// Forward: a workgroup takes 64 query points, a thread adds up the pieces of a slot, then the first 64 threads the slots of a point.
+// Forward: a workgroup takes 64 query points, a thread adds up the pieces of a slot, then the first 64 threads the slots of a point (16384
+// slots: 5.6 us; a thread for each query, adding its slots one after the other, took 5 us more).
 constexpr int kMeanPoints = 64, kMeanThreads = 256;
 __global__ __launch_bounds__(kMeanThreads) void experts_mean_kernel(const JoinArgs a)
 {
@@ -457,7 +466,7 @@ __global__ __launch_bounds__(kMeanThreads) void experts_mean_kernel(const JoinAr
     }
 }
 
-// backward: the gradient of each coefficient from its pieces, of each weight from its slot's mean
+// backward: the gradient of each coefficient from its pieces, of each weight from its slot's mean (32768 points, 8192 slots: 4.2 us, latency)
 __global__ __launch_bounds__(256) void experts_gradient_kernel(const JoinArgs a)
 {
     const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -580,8 +589,11 @@ int fr_experts_predict(fr_ctx* ctx, const fr_kprog* kernel, const double* X, int
         if (out_slots) FR_TRY(os.stage(out_slots, m, k, lds, 8, "out_slots", true));
         if (m == 0) return FR_OK;
         const int64_t slots = m * k;
-        // few slots an expert: sums over lanes of points; many: a lane for each slot (both sides measured: see experts_few_kernel)
-        const bool few = slots < n_experts * 64;
+        // Few slots an expert, or more features than registers hold: sums over lanes of points; else a lane for each slot.  us, the one / the
+        // other, at 32, 64, 128, 192 and 256 slots an expert: 64 experts of 128 points of 16 features 21 / 22, 22 / 24, 28 / 27, 30 / 30,
+        // 36 / 32; 8 of 8192 of 8 features 21 / 49, 28 / 46, 35 / 52, 43 / 52, 55 / 63.  At 256, 1024 and 2048: 64 of 1024 of 16 features 70 /
+        // 76, 219 / 214, 424 / 386; 64 of 128 of 16 features 35 / 32, 105 / 79, 198 / 140; 64 of 1024 of 40 features 115 / 136, 380 / 428, 749 / 820
+        const bool few = d > 16 || slots < n_experts * 192;
         const int64_t used = slots < n_experts ? slots : n_experts, blocks = (slots + 7) / 8 + used, tiles = few ? blocks : slots / kSide + used;
         const int64_t want = (int64_t)ctx->num_cus * (few ? 4 : 20);
         const int64_t piece = piece_rows(want, tiles, n, n_experts, slots, few ? 256 : 8), pieces = n / piece + 2;

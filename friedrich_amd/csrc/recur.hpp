@@ -321,6 +321,11 @@ __device__ __forceinline__ void find_wave_edges(const RecArgs& a, int64_t lo, in
 // a wave holds 64 >> lanes such stretches of rows and the workgroup's waves the rows after them.  UNIFORM: a wave holds one stretch
 // (64 channel lanes), so rows, their addresses and what begins and ends in them are the same for the whole wave and cost no vector
 // instruction; a stretch inside one sequence then runs without a branch.
+//
+// bf16, a gate for 128 channels, 37 sequences of 16413 rows x 2048 channels: backward 203 MB in 84 us, 2.4 TB/s (with vector
+// addresses and edges looked for in every row 113 and more).  The rest is the wait for the maps in front and the tail: a workgroup of 8 waves fills the
+// registers of its CU, so loading, waiting and storing take turns.  3, 4 and 6 waves, windows of 8 and 32 tiles and 128 registers a lane were no
+// faster.  24 sequences of one row: the launch.
 
 template <typename T, int FORM, int V, bool SHARED, bool BACKWARD, bool UNIFORM, bool FEW>
 __global__ __launch_bounds__(512) void rec_rows_kernel(const RecArgs a)
@@ -670,6 +675,10 @@ __global__ __launch_bounds__(512) void rec_rows_kernel(const RecArgs a)
 //
 // A lane holds E neighbouring rows of up to CG channels that share their gate, a workgroup 64 E rows a wave.  The gate is read, and its
 // exponential worked out, once for those channels.
+//
+// f64, three channels on one gate, 1000003 x 3 backward: 112 MB in 32 us, 3.5 TB/s; four on one, 4194307 x 4 forward: 302 MB in 104 us, 2.9 TB/s.
+// Bound as the rows are, by tiles that load, wait and store in turn (with blocks of 256 tiles and a map's words apart for each channel 149; 16 waves of 4
+// rows a lane 99, but 44 instead of 40 where there is one channel).
 
 template <typename T, int FORM, int CG, bool BACKWARD>
 __global__ __launch_bounds__(512) void rec_columns_kernel(const RecArgs a)
@@ -1039,10 +1048,13 @@ static int rec_rows(fr_ctx* ctx, RecArgs& a, bool backward, OpWorkspace& ws)
     };
     if (few)
         hipLaunchKernelGGL((rec_rows_kernel<T, FORM, V, SHARED, false, true, true>), grid, block, 0, ctx->ls, a);
-    else if (V > 1 || a.lanes == 6)
+    else if constexpr (V == 1) {
+        if (a.lanes == 6)
+            launch(std::true_type());
+        else
+            launch(std::false_type());
+    } else if constexpr (SHARED || sizeof(T) == 2)  // (two channels of 32 bits with a gate each: few rows only)
         launch(std::true_type());
-    else if constexpr (V == 1)
-        launch(std::false_type());
     return FR_OK;
 }
 
@@ -1073,7 +1085,15 @@ static bool rec_is_column(const RecArgs& a)
 template <typename T, int FORM>
 static int rec_launch(fr_ctx* ctx, RecArgs& a, int layout, bool backward, OpWorkspace& ws)
 {
-    constexpr int WIDE = 8 / (int)sizeof(T);  // channels of a lane: 8 bytes of them once that fills a wave
+    // A lane of 8 bytes of channels fetches fewer, longer lines and works a shared gate out once; a lane of one channel makes more workgroups
+    // and keeps more rows' data in flight.  Wide once the call is large enough to fill the chip that way, and for few rows, where the
+    // tiles are few either way (bf16, us wide / narrow, shared gate: 4096 x 256 forward 22 / 19, backward 25 / 21; 16384 x 512 26 / 29 and 37 /
+    // 48; 16413 x 2048 backward 83 / 168.  A gate a channel: 4096 x 1024 24 / 23 and 33 / 29; 65536 x 256 64 / 56 and 76 / 75; 16384 x 1024
+    // 49 / 53 and 64 / 72; 1024 x 2048 forward 17 / 26.  f32, a gate a channel: 16384 x 1024 59 / 54 and 87 / 84, 32768 x 1024
+    // 106 / 100 and 152 / 151; shared 16384 x 512 27 / 30 and 41 / 48).
+    constexpr int WIDE = 8 / (int)sizeof(T);
+    const bool few = !backward && a.n <= kFewRows, fits = WIDE > 1 && a.d >= 64 * WIDE && a.d % WIDE == 0 && (a.width == 1 || a.width % WIDE == 0);
+    const bool wide = fits && (few || (a.width > 1 ? a.n * a.d >= 1 << 22 : sizeof(T) == 2 && a.d >= 128 * WIDE && a.n * a.d >= 1 << 23));
     if (layout == FR_LAYOUT_COLMAJOR || rec_is_column(a)) {
         if (a.width == 1)
             FR_TRY((rec_columns<T, FORM, 1>(ctx, a, backward, ws)));
@@ -1081,7 +1101,7 @@ static int rec_launch(fr_ctx* ctx, RecArgs& a, int layout, bool backward, OpWork
             FR_TRY((rec_columns<T, FORM, 2>(ctx, a, backward, ws)));
         else
             FR_TRY((rec_columns<T, FORM, 4>(ctx, a, backward, ws)));
-    } else if (WIDE > 1 && a.d >= 64 * WIDE && a.d % WIDE == 0 && (a.width == 1 || a.width % WIDE == 0)) {
+    } else if (wide) {
         if (a.width == 1)
             FR_TRY((rec_rows<T, FORM, WIDE, false>(ctx, a, backward, ws)));
         else

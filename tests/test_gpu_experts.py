@@ -248,6 +248,22 @@ def test_experts_forward_and_backward(tctx, spec):  # noqa: F811
             assert np.all(np.abs(da - want_a) <= rel * size_a + 1e-300), (n, d, experts, m, k)
 
 
+@pytest.mark.parametrize("spec", SPECS[::3], ids=lambda s: s[0])
+@pytest.mark.parametrize("per_expert", [31, 190, 200, 700])
+def test_experts_on_either_side_of_many_slots(tctx, spec, per_expert):  # noqa: F811
+    """slots an expert around the number from which a lane takes a slot, for features that stay in registers and more of them"""
+    rng = np.random.default_rng(32)
+    for n, d, experts in ((1200, 3, 3), (900, 8, 2), (700, 16, 5), (300, 33, 1)):
+        m = per_expert * experts // 2
+        X, Xq, offsets, chosen, w, alpha = model(rng, n, d, experts, m, 2, unused=0.05)
+        want, want_s, size = P.experts_predict(spec, X, alpha, offsets, Xq, chosen, w, None)
+        rel = (int(np.max(np.diff(offsets))) + (d + 8) * (1 + arg(d)) + 16) * 2 * U
+        x, q, o, c, ww, a = device(X, Xq, offsets, chosen, w, alpha)
+        mean, slots = (host(v) for v in tctx.experts_predict(spec, x, a, o, q, c, ww))
+        assert np.all(np.abs(slots - want_s) <= rel * size + 1e-300), (n, d, experts, m)
+        assert np.all(np.abs(mean - want) <= (rel + 4 * U) * (np.abs(w) * size).sum(1) + 1e-300), (n, d, experts, m)
+
+
 def test_one_expert_is_predict_mean(tctx):  # noqa: F811
     """each expert fitted by fr_chol_from_inputs on its own rows, alpha by fr_chol_solve: the mean of a query that names it alone is
     fr_predict_mean's"""

@@ -147,6 +147,35 @@ def test_gradients_of_one_sequence(tctx, form, dtype, layout):
             check(g, *ref[name], (6 * n + 24 + d // cols) * UNIT[dtype], 0.0 if name == "dh0" else HALF_STEP[dtype], (name, n, d, cols), 0.0 if name == "dh0" else TINY[dtype])
 
 
+@pytest.mark.parametrize("form", ["value", "log", "stationary"])
+@pytest.mark.parametrize("dtype,n,d,cols", [("bf16", 8200, 1024, 1024), ("bf16", 8200, 516, 129), ("f16", 8200, 520, 65), ("f32", 8200, 520, 65), ("f32", 600, 512, 512), ("bf16", 600, 512, 512)])
+def test_several_channels_a_lane(tctx, dtype, n, d, cols, form):
+    """rows layout, calls large enough for (or, of few rows, with) more than one channel a lane; sequences that begin anywhere"""
+    import torch
+
+    t = torch_types()[dtype]
+    rng = np.random.default_rng(15)
+    cuts = [2, 2, 40, 257, 258, n // 2, n // 2 + 128, n - 3]
+    nseq, longest = len(cuts) - 1, n // 2
+    gate, x, h0, wide = problem(rng, n, d, cols, nseq, form, dtype, "row")
+    offsets = torch.tensor(cuts, dtype=torch.int64, device="cuda")
+    h, last = put(np.full((n, d), 7.0), "row", t), put(np.full((nseq, d), 7.0), "row", wide)
+    tctx.recurrence(gate, x, form=form, offsets=offsets, h0=h0, out=h, last=last)
+    want, want_last, z, zl = P.recurrence(form, host(gate), host(x), cuts, host(h0))
+    rel, within = (6 * longest + 8) * UNIT[dtype], slice(cuts[0], cuts[-1])
+    assert (h[: cuts[0]] == 7.0).all() and (h[cuts[-1] :] == 7.0).all()
+    check(h[within], want[within], z[within], rel, HALF_STEP[dtype], "h", TINY[dtype])
+    check(last, want_last, zl, rel, 0.0, "last")
+    dh, dlast = put(rng.standard_normal((n, d)), "row", t), put(rng.standard_normal((nseq, d)), "row", wide)
+    dgate, dx, dh0 = put(np.full((n, cols), 7.0), "row", t), put(np.full((n, d), 7.0), "row", t), put(np.full((nseq, d), 7.0), "row", wide)
+    tctx.recurrence_backward(gate, x, h, dh, form=form, offsets=offsets, h0=h0, dlast=dlast, dgate=dgate, dx=dx, dh0=dh0)
+    ref = P.recurrence_backward(form, host(gate), host(x), host(h), host(dh), cuts, host(h0), host(dlast))
+    for name, got in (("dgate", dgate), ("dx", dx)):
+        assert (got[: cuts[0]] == 7.0).all() and (got[cuts[-1] :] == 7.0).all(), name
+        check(got[within], ref[name][0][within], ref[name][1][within], (6 * longest + 24 + d // cols) * UNIT[dtype], HALF_STEP[dtype], name, TINY[dtype])
+    check(dh0, *ref["dh0"], rel, 0.0, "dh0")
+
+
 def test_gradients_against_differences(tctx):
     """central differences of a scalar loss in f64: error h^2 times a third derivative of the order of the loss, and round-off over h"""
     import torch
