@@ -11,6 +11,7 @@ namespace fr {
 
 constexpr int kMaxExperts = 1024;
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanHeld = 4096;  // slots of an expert whose list stays in LDS
 constexpr int kSide = 64;   // lanes of a wave, one slot (or point) each
 constexpr int kStep = 8;    // points (or slots) that a lane works on at a time
 
@@ -20,7 +21,7 @@ struct PlanArgs {
     const int* chosen;
     const double *Xq, *weights, *dmean;
     int64_t* starts;  // experts + 1: where an expert's slots begin in the list
-    int* list;        // list place -> slot (slot j m + q: the j-th of query q)
+    int* list;        // list place -> slot (slot j m + q: the j-th of query q); experts of more than kPlanHeld slots only
     int* place;       // slot -> its place in the list, -1 unused
     double* packed;   // d x slots, feature-major: query points in list order (null: blocks instead)
     double* blocks;   // ... or blocks of 8 places of the list: 8 (d + 1) doubles, feature by feature, then dmean_q w_qj (backward)
@@ -39,13 +40,13 @@ __device__ __forceinline__ int64_t block_index(int64_t row, int64_t f, int64_t d
 // one, which is where the expert's list begins; a second walk puts each slot in its place, and the workgroup packs its list's query
 // points.  No atomics: a list's order is that of (share, j, q) on every run.  Every workgroup reads all slots (16384 slots: 64 KB, from
 // L2), which costs less than a launch to sort them first.  Bound by
-// latency, the two walks and the packing behind them: 7 us for 6 slots of 16 experts, 15 us for 16384 slots of 64 experts and 65536 points of 16
-// features (8 MB read and written).
+// latency, the two walks and the packing behind them: 6.5 us for 6 slots of 16 experts, 14 us for 16384 slots of 64 experts and 65536 points of 16
+// features (8 MB read and written).  The list stays in LDS where it fits: written to memory and read again it took 1 us more.
 // (loads under a condition are waited for one by one: out of range they read the last place instead)
 __global__ __launch_bounds__(kPlanThreads) void experts_plan_kernel(const PlanArgs a)
 {
     constexpr int WAVES = kPlanThreads / 64;
-    __shared__ int mine[WAVES], before[WAVES];
+    __shared__ int mine[WAVES], before[WAVES], held[kPlanHeld];
     if ((int)blockIdx.x >= a.experts) {
         const int64_t step = (int64_t)(gridDim.x - a.experts) * kPlanThreads;
         for (int64_t i = (int64_t)(blockIdx.x - a.experts) * kPlanThreads + threadIdx.x; i < a.n; i += step) {
@@ -115,7 +116,10 @@ __global__ __launch_bounds__(kPlanThreads) void experts_plan_kernel(const PlanAr
                 if (at[i] == e) {
                     const int p = place + __popcll(all & ((1ull << lane) - 1));
                     a.place[j * a.m + slot] = p;
-                    a.list[p] = (int)(j * a.m) + slot;
+                    if (total <= kPlanHeld)
+                        held[p - start] = (int)(j * a.m) + slot;
+                    else
+                        a.list[p] = (int)(j * a.m) + slot;
                 } else if (e == 0 && slot < hi && (at[i] < 0 || at[i] >= a.experts))
                     a.place[j * a.m + slot] = -1;
                 place += __popcll(all);
@@ -123,7 +127,7 @@ __global__ __launch_bounds__(kPlanThreads) void experts_plan_kernel(const PlanAr
         }
     __syncthreads();  // (the list is this workgroup's own: no other reads or writes its part)
     for (int i = threadIdx.x; i < total; i += kPlanThreads) {
-        const int slot = a.list[start + i], j = slot / m, q = slot - j * m;
+        const int slot = total <= kPlanHeld ? held[i] : a.list[start + i], j = slot / m, q = slot - j * m;
         if (a.dmean) a.blocks[block_index(start + i, fours(a.d), a.d)] = a.dmean[q] * a.weights[q + j * a.ldw];
         if (a.blocks)
             for (int64_t f = a.d; f < fours(a.d); ++f) a.blocks[block_index(start + i, f, a.d)] = 0.0;
@@ -179,21 +183,36 @@ __device__ __forceinline__ int64_t same(int64_t v)
     return (int64_t)((unsigned long long)hi << 32 | lo);
 }
 
-// The covariance from s and u.  Kernels of one length scale multiply by its inverse, worked out once, where the Gram kernel divides: a
-// rounding of the exponent more, which the sum over the points hides, for five instructions less a pair.
+// 2^y for y <= 0, to a rounding or two: the rest of y after its nearest integer is exact, and the series of 2^r about 0 has a remainder of
+// 4e-18 at |r| = 1/2.  A pair of instructions fewer than e^x, and none for large arguments.
+__device__ __forceinline__ double exp2_falling(double y)
+{
+    const double n = __builtin_rint(y), r = y - n;
+    constexpr double C[12] = {2.5678435993488206e-11, 4.4455382718708116e-10, 7.054911620801123e-09, 1.01780860092397e-07,  1.321548679014431e-06, 1.5252733804059841e-05,
+                              0.0001540353039338161,  0.0013333558146428443,  0.009618129107628477,  0.05550410866482158, 0.24022650695910072, 0.6931471805599453};
+    double p = 1.3691488853904128e-12;  // ln(2)^13 / 13!
+#pragma unroll
+    for (int i = 0; i < 12; ++i) p = __builtin_fma(p, r, C[i]);
+    const double e = __builtin_ldexp(__builtin_fma(p, r, 1.0), (int)n);
+    return y < -1080.0 ? 0.0 : e;  // (-inf has no r)
+}
+
+// The covariance from s and u, without the amplitude that kernels of one length scale begin with: it multiplies the sum.  They also multiply by
+// the length's inverse, worked out once, where the Gram kernel divides: a rounding of the exponent more, which the sum over the points
+// hides, for five instructions less a pair.
+constexpr double kLog2e = 1.4426950408889634;
 template <int LEAF>
 __device__ __forceinline__ double pair_value(const fr_kprog& p, double inverse, double s, double u)
 {
-    const double ampl = fabs(p.ops[0].params[1]);
-    if constexpr (LEAF == FR_K_SQUAREDEXP) return ampl * exp_fast(-(s * inverse));
-    if constexpr (LEAF == FR_K_EXPONENTIAL) return ampl * exp_fast(-(sqrt(s) * inverse));
+    if constexpr (LEAF == FR_K_SQUAREDEXP) return exp2_falling(-(s * inverse));
+    if constexpr (LEAF == FR_K_EXPONENTIAL) return exp2_falling(-(sqrt(s) * inverse));
     if constexpr (LEAF == FR_K_MATERN1) {
         const double x = sqrt(s) * inverse;
-        return ampl * (1.0 + x) * exp_fast(-x);
+        return (1.0 + x) * exp2_falling(-(x * kLog2e));
     }
     if constexpr (LEAF == FR_K_MATERN2) {
         const double x = sqrt(s) * inverse;
-        return ampl * __builtin_fma(x, x * (1.0 / 3.0), 1.0 + x) * exp_fast(-x);
+        return __builtin_fma(x, x * (1.0 / 3.0), 1.0 + x) * exp2_falling(-(x * kLog2e));
     }
     return kprog_eval_k<LEAF>(p, s, u);
 }
@@ -201,15 +220,20 @@ template <int LEAF>
 __device__ __forceinline__ double pair_inverse(const fr_kprog& p)
 {
     const double ls = p.ops[0].params[0];
-    if constexpr (LEAF == FR_K_SQUAREDEXP || LEAF == FR_K_EXPONENTIAL) return 1.0 / (2.0 * ls * ls);
+    if constexpr (LEAF == FR_K_SQUAREDEXP || LEAF == FR_K_EXPONENTIAL) return kLog2e / (2.0 * ls * ls);
     if constexpr (LEAF == FR_K_MATERN1) return sqrt(3.0) / fabs(ls);
     if constexpr (LEAF == FR_K_MATERN2) return sqrt(5.0) / fabs(ls);  // 5 s / (3 ls^2) = x^2 / 3
     return 0.0;
 }
+template <int LEAF>
+__device__ __forceinline__ double pair_scale(const fr_kprog& p)
+{
+    return LEAF == FR_K_SQUAREDEXP || LEAF == FR_K_EXPONENTIAL || LEAF == FR_K_MATERN1 || LEAF == FR_K_MATERN2 ? fabs(p.ops[0].params[1]) : 1.0;
+}
 
 // kStep covariances of the lane's point with the points of a block.  The distance is summed from the differences, feature by feature, as the
 // Gram kernel does: |x|^2 + |y|^2 - 2 x.y on the matrix cores would lose near points' distances to cancellation, which the square root in
-// three of the kernels turns into an error of 1e-8.  That makes 2 d + about 28 f64 instructions a pair, at 4 cycles a wave and SIMD.  The
+// three of the kernels turns into an error of 1e-8.  That makes 2 d + about 22 f64 instructions a pair, at 4 cycles a wave and SIMD.  The
 // block comes through scalar loads of one line each, eight points of a feature: it costs no vector register and no LDS traffic (a broadcast
 // read of LDS for every 16 instructions would keep the LDS pipe of the CU busier than its SIMDs), and a block is contiguous, so its
 // lines need one address.
@@ -297,8 +321,8 @@ __device__ __forceinline__ int expert_of(const BlockArgs& a, const int64_t* item
 // A lane for each row of the columns' side, the sum over the blocks: an item is a wave of 64 lanes times a piece of blocks.  FOURS > 0: the
 // lanes' features stay in registers; 0: there are more than 16, and they are read again for every block.  Bound by issue of f64
 // instructions: 16777216 pairs of 16 features (squared exponential, 64 experts of 500 to 1500 points) take
-// 61 us, where 60 instructions a pair would take 26; 7500000 in the backward pass 33 us.  20 items a CU even skewed experts out: whole
-// calls with 5, 10, 20 and 32 took 114, 86, 77 and 75 us, backward 49, 45, 44 and 45.
+// 51 us, where 54 instructions a pair would take 23; 7500000 in the backward pass 27 us.  40 items a CU, on no more workgroups than the chip
+// holds, even skewed experts out: whole calls with 20 items on 8 workgroups took 74 and 41 us, with 40 on 5 70 and 39, with 80 on 5 75 and 48.
 template <int LEAF, int FOURS>
 __global__ __launch_bounds__(256) void experts_lanes_kernel(const BlockArgs a)
 {
@@ -350,14 +374,14 @@ __global__ __launch_bounds__(256) void experts_lanes_kernel(const BlockArgs a)
                     if (j + t >= b0 && j + t < to) acc = __builtin_fma(pair_value<LEAF>(a.prog, inverse, p.s[t], p.u[t]), v[t], acc);
             }
         }
-        if (row < r1) a.part[row + piece * a.rows] = acc;
+        if (row < r1) a.part[row + piece * a.rows] = acc * pair_scale<LEAF>(a.prog);
     }
 }
 
 // A lane for each row of the columns' side too, but the sum is over the lanes: an item is a block of 8 slots times a piece of the expert's
 // points, which the four waves share out; the points' features are read again for every block.  For few slots an expert, where lanes of slots
-// would be empty, and for many features (16 experts of 1024 points of 16
-// features, 3 queries of 2 slots: 7 us, most of it latency; 16777216 pairs of 40 features: 102 us, issue).  4 items a CU: with 2, 512 queries
+// would be empty (16 experts of 1024 points of 16
+// features, 3 queries of 2 slots: 7 us, most of it latency).  4 items a CU: with 2, 512 queries
 // of 40 features took 33 us instead of 29, 8 took as long.
 template <int LEAF>
 __global__ __launch_bounds__(256) void experts_few_kernel(const BlockArgs a)
@@ -404,7 +428,8 @@ __global__ __launch_bounds__(256) void experts_few_kernel(const BlockArgs a)
             for (int t = 0; t < kStep; ++t) sums[wave][t] = acc[t];
         __syncthreads();
         if (threadIdx.x < kStep && j + threadIdx.x >= b0 && j + threadIdx.x < b1)
-            a.part[j + threadIdx.x + piece * a.block_rows] = ((sums[0][threadIdx.x] + sums[1][threadIdx.x]) + sums[2][threadIdx.x]) + sums[3][threadIdx.x];
+            a.part[j + threadIdx.x + piece * a.block_rows] =
+                (((sums[0][threadIdx.x] + sums[1][threadIdx.x]) + sums[2][threadIdx.x]) + sums[3][threadIdx.x]) * pair_scale<LEAF>(a.prog);
         __syncthreads();
     }
 }
@@ -436,7 +461,7 @@ __device__ __forceinline__ double add_pieces(const double* part, int64_t ld, int
 }
 
 // Forward: a workgroup takes 64 query points, a thread adds up the pieces of a slot, then the first 64 threads the slots of a point (16384
-// slots: 5.6 us; a thread for each query, adding its slots one after the other, took 5 us more).
+// slots: 8 us; a thread for each query, adding its slots one after the other, took 5 us more).
 constexpr int kMeanPoints = 64, kMeanThreads = 256;
 __global__ __launch_bounds__(kMeanThreads) void experts_mean_kernel(const JoinArgs a)
 {
@@ -520,8 +545,8 @@ static void leaf_launch(fr_ctx* ctx, const BlockArgs& a, dim3 grid)
 template <bool FEW>
 static int block_launch(fr_ctx* ctx, const BlockArgs& a, int64_t items)
 {
-    // a workgroup for each item if the experts are alike (any number of them finishes the list), no more than the chip holds
-    const int64_t cap = (int64_t)ctx->num_cus * 8;
+    // a workgroup for each item if the experts are alike (any number of them finishes the list), no more than the chip holds: 4 or 5 waves a SIMD
+    const int64_t cap = (int64_t)ctx->num_cus * 5;
     const dim3 grid((unsigned)round_up(items < 1 ? 1 : (items < cap ? items : cap), 8));
     const int leaf = a.prog.nops == 1 ? a.prog.ops[0].kind : -1;
 #define FR_EXPERTS_LEAF(KIND) \
@@ -589,13 +614,13 @@ int fr_experts_predict(fr_ctx* ctx, const fr_kprog* kernel, const double* X, int
         if (out_slots) FR_TRY(os.stage(out_slots, m, k, lds, 8, "out_slots", true));
         if (m == 0) return FR_OK;
         const int64_t slots = m * k;
-        // Few slots an expert, or more features than registers hold: sums over lanes of points; else a lane for each slot.  us, the one / the
-        // other, at 32, 64, 128, 192 and 256 slots an expert: 64 experts of 128 points of 16 features 21 / 22, 22 / 24, 28 / 27, 30 / 30,
-        // 36 / 32; 8 of 8192 of 8 features 21 / 49, 28 / 46, 35 / 52, 43 / 52, 55 / 63.  At 256, 1024 and 2048: 64 of 1024 of 16 features 70 /
-        // 76, 219 / 214, 424 / 386; 64 of 128 of 16 features 35 / 32, 105 / 79, 198 / 140; 64 of 1024 of 40 features 115 / 136, 380 / 428, 749 / 820
-        const bool few = d > 16 || slots < n_experts * 192;
+        // Few slots an expert: sums over lanes of points; else a lane for each slot.  us, the one / the other, at 32, 64, 128, 192 and 256 slots an
+        // expert: 64 experts of 128 points of 16 features 20 / 21, 20 / 24, 26 / 26, 29 / 29, 34 / 33; 8 of 8192 of 8 features 20 / 60,
+        // 26 / 65, 33 / 58, 40 / 58, 51 / 61; at 64, 128, 192, 256 and 1024: 64 of 1024 of 16 features 39 / 44, 47 / 51, 57 / 59, 65 / 67,
+        // 221 / 185; of 40 features at 256 and 1024 110 / 119, 403 / 393
+        const bool few = slots < n_experts * 256;
         const int64_t used = slots < n_experts ? slots : n_experts, blocks = (slots + 7) / 8 + used, tiles = few ? blocks : slots / kSide + used;
-        const int64_t want = (int64_t)ctx->num_cus * (few ? 4 : 20);
+        const int64_t want = (int64_t)ctx->num_cus * (few ? 4 : 40);
         const int64_t piece = piece_rows(want, tiles, n, n_experts, slots, few ? 256 : 8), pieces = n / piece + 2;
         const int64_t wide = 8 * (fours(d) + 1);
         OpWorkspace ws(ctx);
@@ -660,7 +685,7 @@ int fr_experts_backward(fr_ctx* ctx, const fr_kprog* kernel, const double* X, in
         OpWorkspace ws(ctx);
         if (dalpha && n > 0) {
             const int64_t used = n < n_experts ? n : n_experts, blocks = (slots + 7) / 8 + 1, tiles = n / kSide + used;
-            const int64_t piece = piece_rows((int64_t)ctx->num_cus * 20, tiles, slots, n_experts, n, 8), pieces = slots / piece + 2;
+            const int64_t piece = piece_rows((int64_t)ctx->num_cus * 40, tiles, slots, n_experts, n, 8), pieces = slots / piece + 2;
             FR_TRY(ws.get((size_t)(8 * (blocks * 8 * (fours(d) + 1) + pieces * n + n_experts + 1) + 8 * slots)));
             PlanArgs p = {};
             p.m = m, p.k = k, p.slots = slots, p.d = d, p.ldq = oq.ld, p.lde = oe.ld, p.ldw = ow.ld, p.experts = (int)n_experts;

@@ -264,6 +264,43 @@ def test_experts_on_either_side_of_many_slots(tctx, spec, per_expert):  # noqa: 
         assert np.all(np.abs(mean - want) <= (rel + 4 * U) * (np.abs(w) * size).sum(1) + 1e-300), (n, d, experts, m)
 
 
+def test_experts_of_thousands_of_slots(tctx):  # noqa: F811
+    """lists of one expert on either side of what a workgroup holds, beside experts with none, one and few slots"""
+    rng = np.random.default_rng(33)
+    spec = ("matern2", 0.9, 1.2)
+    for n, d, experts, m, k in ((60, 3, 1, 4096, 1), (60, 3, 1, 4097, 1), (90, 17, 4, 3000, 2), (40, 2, 2, 9001, 1)):
+        X, Xq, offsets, chosen, w, alpha = model(rng, n, d, experts, m, k)
+        chosen[chosen == experts - 1] = 0
+        if experts > 1:
+            chosen[5, 0] = experts - 1
+        dmean = rng.standard_normal(m)
+        want, want_s, size = P.experts_predict(spec, X, alpha, offsets, Xq, chosen, w, None)
+        x, q, o, c, ww, a, dm, ws = device(X, Xq, offsets, chosen, w, alpha, dmean, np.asfortranarray(want_s))
+        mean, slots = (host(v) for v in tctx.experts_predict(spec, x, a, o, q, c, ww))
+        rel = (int(np.max(np.diff(offsets))) + (d + 8) * (1 + arg(d)) + 16) * 2 * U
+        assert np.all(np.abs(slots - want_s) <= rel * size + 1e-300), (n, d, experts, m)
+        assert np.all(np.abs(mean - want) <= (rel + 4 * U) * (np.abs(w) * size).sum(1) + 1e-300), (n, d, experts, m)
+        want_w, want_a, size_a = P.experts_backward(spec, X, offsets, Xq, chosen, w, want_s, dmean)
+        dw, da = (host(v) for v in tctx.experts_backward(spec, x, o, q, c, ww, ws, dm))
+        assert np.all(np.abs(dw - want_w) <= 2 * U * np.abs(want_w)), (n, d, experts, m)
+        assert np.all(np.abs(da - want_a) <= (m * k + (d + 8) * (1 + arg(d)) + 16) * 2 * U * size_a + 1e-300), (n, d, experts, m)
+
+
+def test_covariances_that_vanish(tctx):  # noqa: F811
+    """distances from none to beyond the smallest covariance, infinite and undefined ones: 0 and NaN as the Gram kernel has them, subnormals
+    within the smallest step (half of it on either side), the exponent's error as in the other tests"""
+    for name, reach in (("squared_exp", 40.0), ("exponential", 1600.0), ("matern1", 500.0), ("matern2", 400.0)):
+        spec = (name, 1.0, 1.5)
+        Xq = np.concatenate([np.linspace(0.0, reach, 400), [np.inf, np.nan]]).reshape(-1, 1)
+        m = len(Xq)
+        chosen, w = np.zeros((m, 1), np.int32, order="F"), np.ones((m, 1), order="F")
+        got, _ = tctx.experts_predict(spec, np.zeros((1, 1)), np.ones(1), np.array([0, 1]), Xq, chosen, w)
+        want = tctx.gram(spec, Xq, np.zeros((1, 1)))[:, 0]
+        assert np.array_equal(np.isnan(got), np.isnan(want)) and np.isnan(got[-1])
+        ok = ~np.isnan(want)
+        assert np.all(np.abs(got - want)[ok] <= 16 * 800 * 2 * U * want[ok] + 2.0**-1074)
+
+
 def test_one_expert_is_predict_mean(tctx):  # noqa: F811
     """each expert fitted by fr_chol_from_inputs on its own rows, alpha by fr_chol_solve: the mean of a query that names it alone is
     fr_predict_mean's"""
