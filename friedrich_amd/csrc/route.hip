@@ -392,8 +392,10 @@ __global__ __launch_bounds__(256, 2) void route_lists_kernel(const RouteArgs a)
     const int64_t turns = (a.n + (256 >> a.lanes) - 1) / (256 >> a.lanes);
     const bool grouped = a.top_groups < a.groups;
     const bool scored = a.bias || grouped;  // the order needs the scores
-    // Error of a 32-bit score, of at most 1: the exponential is good to 2 ulp and |x| 2^-24 of its argument, which a sigmoid's slope turns into
-    // at most 2^-22 altogether; a softmax adds the rounding of the sum of its up to 16 terms a lane, 2^-20.  Adding a bias rounds twice.
+    // Error of a 32-bit score, of at most 1: the exponential is good to 2 ulp and |x| 2^-23 of its argument x, which a sigmoid's slope turns into
+    // at most 2^-22 altogether; a softmax adds the rounding of the sum of its up to 16 terms a lane, 2^-20.  Adding a bias rounds twice.  x is a
+    // logit (sigmoid, where |x| is paid for by the slope) or its distance from the row's largest, taken in the wide type: that of two
+    // rounded logits would be off by a part of the logits, which a row may have as large as it likes.
     constexpr float kNear = SIGMOID ? 0x1p-21f : 0x1p-19f;
     const float near_key = a.bias ? 2.0f * kNear : 0.0f;  // for two keys, times 1 + |key| (f64 logits rounded to 32 bits keep their order)
     const bool exact = sizeof(T) < 8 && !a.bias;
@@ -443,7 +445,7 @@ __global__ __launch_bounds__(256, 2) void route_lists_kernel(const RouteArgs a)
             } else if (scored) {
                 float sum = 0.0f;
 #pragma unroll
-                for (int c = 0; c < C; ++c) sum += top > -INFINITY ? __expf(key[c] - (float)top) : 0.0f;
+                for (int c = 0; c < C; ++c) sum += top > -INFINITY ? __expf((float)(widen(raw[c]) - top)) : 0.0f;
                 sum = at.lane_sum(sum);
                 about = sum > 0.0f ? 1.0f / sum : 0.0f;
             }
@@ -453,7 +455,7 @@ __global__ __launch_bounds__(256, 2) void route_lists_kernel(const RouteArgs a)
             float rank[C], best = -INFINITY, second = -INFINITY;
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const float sc = SIGMOID ? __builtin_amdgcn_rcpf(1.0f + __expf(-key[c])) : __expf(key[c] - (float)top) * about;
+                const float sc = SIGMOID ? __builtin_amdgcn_rcpf(1.0f + __expf(-key[c])) : __expf((float)(widen(raw[c]) - top)) * about;
                 rank[c] = key[c] == -INFINITY ? key[c] : sc + bias[c];
                 second = fmaxf(second, fminf(best, rank[c]));
                 best = fmaxf(best, rank[c]);

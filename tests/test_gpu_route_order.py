@@ -1,0 +1,61 @@
+"""The order of the experts over many rows, where 32-bit keys decide most of them: logits that 32 bits hold badly or not at all.  Choices
+have to be those of the definition in 64 bits; only rows in which two 64-bit values that decide lie within the exponentials' own error
+(numpy's and the kernel's, an ulp each: 1e-15 (1 + |value|)) may fall either way."""
+import numpy as np
+import pytest
+
+import plain_operators as P
+from test_gpu_recurrence import host, put, tctx, torch_types  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def expected(score, x, bias, groups, kept, k):
+    """-> (experts n x k, rows that rounding may decide)"""
+    n, experts = x.shape
+    p = P.scores(score, x)
+    rank = p + (0.0 if bias is None else bias)
+    closed = np.isneginf(x) | (np.zeros(experts, bool) if bias is None else np.isneginf(bias))
+    rank = np.where(closed, -np.inf, rank)
+    key = np.where(closed, -np.inf, x) if bias is None else rank
+    tight = np.zeros(n, bool)
+    if kept < groups:
+        two = -np.sort(-rank.reshape(n, groups, -1), axis=2)[:, :, :2]
+        value = two[:, :, 0] + (0.0 if two.shape[2] == 1 else np.where(np.isneginf(two[:, :, 1]), 0.0, two[:, :, 1]))
+        best = np.argsort(-value, axis=1, kind="stable")
+        v = np.take_along_axis(value, best, 1)
+        with np.errstate(invalid="ignore"):
+            gap = v[:, kept - 1] - v[:, kept]
+        tight |= (gap != 0) & (gap < 4e-15 * (1 + np.abs(v[:, kept - 1])))
+        open_ = np.zeros((n, groups), bool)
+        np.put_along_axis(open_, best[:, :kept], True, 1)
+        key = np.where(np.repeat(open_, experts // groups, axis=1), key, -np.inf)
+    order = np.argsort(-key, axis=1, kind="stable")
+    lead = np.take_along_axis(key, order, 1)[:, :k + 1]
+    if bias is not None:  # (logits order exactly)
+        with np.errstate(invalid="ignore"):
+            gaps = lead[:, :-1] - lead[:, 1:]
+            tight |= ((gaps > 0) & (gaps < 2e-15 * (1 + np.abs(lead[:, :-1])))).any(1)
+    return np.where(np.isneginf(lead[:, :k]), -1, order[:, :k]), tight
+
+
+def compare(tctx, logits, bias, score, groups, kept, k, what):  # noqa: F811
+    import torch
+
+    got, w = tctx.route(logits, k, score=score, bias=None if bias is None else torch.from_numpy(bias).cuda(), groups=groups, top_groups=kept)
+    want, tight = expected(score, host(logits), bias, groups, kept, k)
+    same = (got.cpu().numpy() == want).all(1)
+    assert (same | tight).all(), (what, int((~(same | tight)).sum()), np.nonzero(~(same | tight))[0][:3], int(tight.sum()))
+    assert tight.sum() < len(want) / 100, (what, int(tight.sum()))
+    return got, w
+
+
+@pytest.mark.parametrize("offset", [-5000.0, 1e4, -1e5, 1e6])
+@pytest.mark.parametrize("experts,k,groups,kept", [(8, 2, 1, 1), (64, 8, 1, 1), (64, 2, 8, 2), (256, 4, 4, 1)])
+def test_far_logits(tctx, experts, k, groups, kept, offset):  # noqa: F811
+    """a softmax does not change when every logit of a row moves by the same amount, as those of squared distances do"""
+    rng = np.random.default_rng(41)
+    n = 32768
+    logits = put(offset + 2.0 * rng.standard_normal((n, experts)), "row", torch_types()["f64"])
+    for bias in ([None] if groups > 1 else []) + [0.1 * rng.standard_normal(experts)]:
+        compare(tctx, logits, bias, "softmax", groups, kept, k, (experts, k, groups, offset, bias is None))
