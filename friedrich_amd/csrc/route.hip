@@ -427,9 +427,9 @@ __global__ __launch_bounds__(256, 2) void route_lists_kernel(const RouteArgs a)
             key[c] = (float)v;
         }
         bool odd = wild;
-        if constexpr (sizeof(T) == 8)  // (what 32 bits would turn into a closed expert)
+        if constexpr (sizeof(T) == 8)  // (what 32 bits would turn into a closed expert, or into one infinite key among others)
 #pragma unroll
-            for (int c = 0; c < C; ++c) odd |= key[c] == -INFINITY && raw[c] != -INFINITY;
+            for (int c = 0; c < C; ++c) odd |= isinf(key[c]) && !isinf(raw[c]);
         double inverse = 1.0;
         float about = 1.0f;  // 1 / the sum of exponentials in 32 bits
         if constexpr (!SIGMOID) {

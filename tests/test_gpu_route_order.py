@@ -59,3 +59,23 @@ def test_far_logits(tctx, experts, k, groups, kept, offset):  # noqa: F811
     logits = put(offset + 2.0 * rng.standard_normal((n, experts)), "row", torch_types()["f64"])
     for bias in ([None] if groups > 1 else []) + [0.1 * rng.standard_normal(experts)]:
         compare(tctx, logits, bias, "softmax", groups, kept, k, (experts, k, groups, offset, bias is None))
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("k", [1, 2, 8])
+def test_logits_beyond_32_bits(tctx, score, k):  # noqa: F811
+    """64-bit logits larger than any of 32 bits, among the slots and just behind the last"""
+    rng = np.random.default_rng(42)
+    n, experts = 20000, 16
+    z = rng.standard_normal((n, experts))
+    huge = np.array([1e39, 2e39, 1e200, 1e300, np.finfo(np.float64).max])
+    for r in range(0, n, 2):
+        at = rng.permutation(experts)[:1 + r % 9]
+        z[r, at] = huge[rng.integers(0, len(huge), len(at))]
+    logits = put(z, "row", torch_types()["f64"])
+    got, w = compare(tctx, logits, None, score, 1, 1, k, (score, k))
+    assert np.isfinite(host(w)).all()
+    if score == "softmax" and k == 1:
+        assert np.all(host(w) == 1.0)  # (renormalised: the largest has all of it)
+    compare(tctx, logits, None, score, 4, 2, k, (score, k, "groups"))
+    compare(tctx, logits, 0.1 * rng.standard_normal(experts), score, 1, 1, k, (score, k, "bias"))
