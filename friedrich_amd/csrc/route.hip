@@ -462,9 +462,8 @@ __global__ __launch_bounds__(256, 2) void route_lists_kernel(const RouteArgs a)
             }
             bool kept = true;
             if (grouped) kept = groups_ahead(a, at, best, second, 4 * kNear, odd) < a.top_groups;  // (two keys in a value)
-            const float shut = kept ? 0.0f : -INFINITY;
 #pragma unroll
-            for (int c = 0; c < C; ++c) key[c] = (a.bias ? rank[c] : key[c]) + shut;
+            for (int c = 0; c < C; ++c) key[c] = !kept ? -INFINITY : (a.bias ? rank[c] : key[c]);  // (a key may be infinite: nothing is added to it)
         }
         double list[K];
 #pragma unroll

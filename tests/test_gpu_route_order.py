@@ -79,3 +79,20 @@ def test_logits_beyond_32_bits(tctx, score, k):  # noqa: F811
         assert np.all(host(w) == 1.0)  # (renormalised: the largest has all of it)
     compare(tctx, logits, None, score, 4, 2, k, (score, k, "groups"))
     compare(tctx, logits, 0.1 * rng.standard_normal(experts), score, 1, 1, k, (score, k, "bias"))
+
+
+@pytest.mark.parametrize("dtype", ["f64", "f32", "bf16"])
+def test_infinite_logits_in_groups(tctx, dtype):  # noqa: F811
+    """a sigmoid of +inf is 1: an expert like any other, shut out with its group where that is not kept"""
+    rng = np.random.default_rng(43)
+    n, experts, groups, kept, k = 20000, 16, 4, 2, 4
+    z = rng.standard_normal((n, experts))
+    z[::2, 4:8] = -9.0
+    z[::2, 5] = np.inf
+    z[1::4, 9] = np.inf
+    logits = put(z, "row", torch_types()[dtype])
+    for layout in ("row", "col"):
+        compare(tctx, put(z, layout, torch_types()[dtype]), None, "sigmoid", groups, kept, k, (dtype, layout))
+    # (the rows do shut it out)
+    want, _ = expected("sigmoid", host(logits), None, groups, kept, k)
+    assert (want[::2] != 5).all(1).sum() > n // 8
