@@ -397,7 +397,7 @@ int fr_markov_product(fr_ctx* ctx, const fr_kprog* kernel, const double* t, int6
 /* Routing of n rows to n_experts <= 1024 experts.  Scores of a row's logits: FR_SCORE_SOFTMAX over all experts, or FR_SCORE_SIGMOID
  * one by one.  An expert of logit -inf is closed to the row.  The experts are ordered by their score + bias (bias: n_experts values; NULL:
  * by their logits), worked out in 64 bits, of equal ones the lower index first; the bias moves the choice only, never a weight, and a
- * NaN bias closes its expert.  With n_groups > 1 (<= 64, dividing n_experts: groups of neighbouring experts) only the experts of
+ * bias of NaN or -inf closes its expert.  With n_groups > 1 (<= 64, dividing n_experts: groups of neighbouring experts) only the experts of
  * the top_groups best groups stay open; a group's value is the sum of its two largest score + bias.  experts (n x k): the k <= 64 best,
  * best first; weights (n x k, wide): scale times their scores, divided by the scores' sum if renormalise (0 where that sum is 0).  Slots
  * for which nothing open is left: expert -1, weight 0.  A row with a NaN logit, or under softmax one of +inf: all slots -1, weights NaN.

@@ -96,3 +96,22 @@ def test_infinite_logits_in_groups(tctx, dtype):  # noqa: F811
     # (the rows do shut it out)
     want, _ = expected("sigmoid", host(logits), None, groups, kept, k)
     assert (want[::2] != 5).all(1).sum() > n // 8
+
+
+@pytest.mark.parametrize("n", [50, 20000])
+def test_a_bias_of_minus_infinity_closes(tctx, n):  # noqa: F811
+    """as a NaN does: no slot, no part in its group's value, whatever else is left"""
+    import torch
+
+    rng = np.random.default_rng(44)
+    experts = 12
+    bias = 0.1 * rng.standard_normal(experts)
+    bias[[0, 3, 4, 5, 6, 7, 9]] = -np.inf  # (the second group of four has none open)
+    logits = put(rng.standard_normal((n, experts)), "row", torch_types()["f32"])
+    for score in ("softmax", "sigmoid"):
+        got, w = compare(tctx, logits, bias, score, 1, 1, 8, score)
+        assert (got[:, 5:] == -1).all() and (w[:, 5:] == 0).all() and (got[:, :5] >= 0).all()
+        got, w = compare(tctx, logits, bias, score, 3, 2, 8, (score, "groups"))
+        assert (got[:, 5:] == -1).all() and (got[:, :5] >= 0).all()
+        nan, _ = tctx.route(logits, 8, score=score, bias=torch.from_numpy(np.where(np.isinf(bias), np.nan, bias)).cuda(), groups=3, top_groups=2)
+        assert torch.equal(nan, got)
