@@ -192,17 +192,31 @@ __device__ __forceinline__ unsigned claim_tile(const RecArgs& a, unsigned* slot)
 
 // the map of a stretch of rows; cut: a sequence begins in it, and nothing in front of it counts (an A of 0 would turn an infinite state
 // of the sequence before into a NaN of this one)
+//
+// A is a product of gates that may leave the type's range where no state does: gates beyond 1 over many rows.  What such an infinite A is
+// multiplied by may be 0 row by row -- a state of 0, or an A of 0 in front of it (a gate of 0 forgets) -- and then stays 0: the rows' own
+// values are in H, and inf * 0 would be a NaN of none of them.
+template <typename S>
+__device__ __forceinline__ S apply(S A, S state, S H)
+{
+    return state == S(0) ? H : A * state + H;
+}
+template <typename S>
+__device__ __forceinline__ S chain(S first, S then)
+{
+    return first == S(0) ? first : first * then;
+}
 template <typename S>
 struct Map {
     S A, H;
     bool cut;
-    __device__ __forceinline__ S of(S state) const { return cut ? H : A * state + H; }
+    __device__ __forceinline__ S of(S state) const { return cut ? H : apply(A, state, H); }
 };
 // first p, then q
 template <typename S>
 __device__ __forceinline__ Map<S> join(const Map<S>& p, const Map<S>& q)
 {
-    return {q.A * p.A, q.of(p.H), p.cut || q.cut};
+    return {chain(p.A, q.A), q.of(p.H), p.cut || q.cut};
 }
 template <typename S>
 __device__ __forceinline__ Map<S> shift_up(const Map<S>& m, int step)
@@ -801,10 +815,10 @@ __global__ __launch_bounds__(512) void rec_columns_kernel(const RecArgs a)
 #pragma unroll
         for (int j = 0; j < CG; ++j) {
             const S ph = __shfl_up(H[j], d);
-            if (lane >= d && !cut) H[j] = A * ph + H[j];
+            if (lane >= d && !cut) H[j] = apply(A, ph, H[j]);
         }
         if (lane >= d) {
-            A *= pa;
+            A = chain(pa, A);
             cut = cut || pc;
         }
     }
@@ -873,7 +887,7 @@ __global__ __launch_bounds__(512) void rec_columns_kernel(const RecArgs a)
         if (j >= ng) continue;
         S st = front[j];
         for (int k = 0; k < wave; ++k) st = Map<S>{mapA[k], mapH[j][k], mapC[k] != 0}.of(st);
-        state[j] = cut ? H[j] : A * st + H[j];
+        state[j] = cut ? H[j] : apply(A, st, H[j]);
     }
 
     if constexpr (!BACKWARD) {

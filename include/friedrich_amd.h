@@ -375,7 +375,10 @@ typedef enum { FR_F64 = 0, FR_F32 = 1, FR_BF16 = 2, FR_F16 = 3 } fr_dtype;
  * outside all sequences are neither read for a result nor written.  offsets == NULL: one sequence of n rows (nseq == 1).  Offsets in
  * device memory are not checked: rows outside [0, n] are never touched, the results of offsets out of order are undefined.
  * h0 (nseq x d, wide; NULL: zeros) is the state in front of each sequence, h_last (nseq x d, wide; may be NULL) the one behind it -- h0
- * itself for a sequence without rows.  h may be x, with the same leading dimension. */
+ * itself for a sequence without rows.  h may be x, with the same leading dimension.
+ * Gates are any numbers, beyond 1 and below 0 too.  Stretches of rows are joined through the product of their gates, in the wide type.
+ * Where that product overflows, a state other than 0 in front of the stretch comes through as infinite or NaN, and where it underflows, not
+ * at all -- also where, row by row, a very small state or later gates would have kept it finite.  A state of 0 stays 0. */
 typedef enum { FR_GATE_VALUE = 0, FR_GATE_LOG = 1, FR_GATE_STATIONARY = 2 } fr_gate;
 int fr_recurrence(fr_ctx* ctx, int dtype, int layout, int form, int64_t n, int64_t d, const void* gate, int64_t gate_cols, int64_t ldg,
                   const void* x, int64_t ldx, const void* offsets, int64_t nseq, const void* h0, int64_t ldh0, void* h, int64_t ldh,
