@@ -983,7 +983,30 @@ __global__ __launch_bounds__(512) void rec_columns_kernel(const RecArgs a)
     }
 }
 
-// dgate of a shared gate from its parts, in the order of the channels
+// The sum of a gate's parts, as many as it has channels where their number fits no wave: thousands of terms that may all round the same way.
+// Parts of 32 bits are summed in 64; of 64 bits each addition's error is kept and added at the end (two-sum).  Either way the sum adds a
+// few roundings whatever the number of parts, as the tree over a wave's lanes does.
+template <typename S>
+struct Total;
+template <>
+struct Total<float> {
+    double v = 0.0;
+    __device__ __forceinline__ void add(float x) { v += (double)x; }
+    __device__ __forceinline__ float get() const { return (float)v; }
+};
+template <>
+struct Total<double> {
+    double v = 0.0, rest = 0.0;
+    __device__ __forceinline__ void add(double x)
+    {
+        const double s = v + x, b = s - v;
+        rest += (v - (s - b)) + (x - b);
+        v = s;
+    }
+    __device__ __forceinline__ double get() const { return isfinite(v) ? v + rest : v; }
+};
+
+// dgate of a shared gate from its parts, in one order on every run
 template <typename T>
 __global__ __launch_bounds__(256) void rec_heads_kernel(const RecArgs a)
 {
@@ -993,9 +1016,13 @@ __global__ __launch_bounds__(256) void rec_heads_kernel(const RecArgs a)
         const int64_t r = a.part_r == 1 ? id % a.n : id / a.cols, q = a.part_r == 1 ? id / a.n : id % a.cols;
         if (r < lo || r >= hi) continue;
         const S* p = (const S*)a.part + r * a.part_r + q * a.pieces * a.part_c;
-        S sum = S(0);
-        for (int64_t i = 0; i < a.pieces; ++i) sum += p[i * a.part_c];
-        ((T*)a.dgate)[r * a.dg_r + q * a.dg_c] = narrow<T>(sum);
+        Total<S> sum[4];  // (four chains: an addition and its error take four dependent instructions)
+        int64_t i = 0;
+        for (; i + 4 <= a.pieces; i += 4)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[k].add(p[(i + k) * a.part_c]);
+        for (; i < a.pieces; ++i) sum[0].add(p[i * a.part_c]);
+        ((T*)a.dgate)[r * a.dg_r + q * a.dg_c] = narrow<T>((sum[0].get() + sum[1].get()) + (sum[2].get() + sum[3].get()));
     }
 }
 

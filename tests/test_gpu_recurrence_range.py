@@ -1,4 +1,4 @@
-"""fr_recurrence where gates grow.  Bounds as in
+"""fr_recurrence where gates grow, and gates shared by numbers of channels that no workgroup's lanes divide.  Bounds as in
 test_gpu_recurrence.py: (6 L + 8) u of the terms' size for L rows, 16 u more backward, and what is said at a test."""
 import numpy as np
 import pytest
@@ -59,3 +59,22 @@ def test_a_forgotten_state_does_not_grow(tctx, layout, d, cols):  # noqa: F811
         assert (h[at:n - 20] == 0).all(), (n, at)
         check(h, want, z, 8 * 64 * UNIT["f32"], 0.0, ("h", n, at), TINY["f32"])
         check(last, want_last, zl, 128 * UNIT["f32"], 0.0, ("last", n, at))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f64"])
+@pytest.mark.parametrize("layout,n,d,cols", [("row", 3, 3000, 1), ("row", 5, 2000, 2), ("row", 1400, 3000, 1), ("row", 9, 4097, 1), ("col", 40, 4097, 1), ("col", 700, 1002, 1)])
+def test_gates_of_thousands_of_channels(tctx, dtype, layout, n, d, cols):  # noqa: F811
+    """the gradient of a gate that many channels share, terms all alike (a running sum of them rounds the same way every time: thousands of
+    half steps).  A term is off by the gate's 4 u twice and five roundings, those it carries from rows behind it weigh a / (1 - a)^2 = 0.06 of 6 u a
+    row; the sum may add the roundings of a tree: 6 of a wave and 8 of the parts.  Together less than 32 u."""
+    t = torch_types()
+    wide = t["f64"] if dtype == "f64" else t["f32"]
+    gate = put(np.full((n, cols), -3.0), layout, t[dtype])
+    h, dh, h0 = put(np.full((n, d), 1.1), layout, t[dtype]), put(np.full((n, d), 0.7), layout, t[dtype]), put(np.full((1, d), 1.3), layout, wide)
+    dg, _, _ = tctx.recurrence_backward(gate, None, h, dh, form="log", h0=h0)
+    g, want = 0.0, np.empty((n, cols))
+    a, y = np.exp(-3.0), float(dh[0, 0])
+    for r in range(n - 1, -1, -1):
+        g = y + a * g
+        want[r] = (d // cols) * (g * float(h[0, 0] if r else h0[0, 0]) * a)
+    check(dg, want, want, 32 * UNIT[dtype], HALF_STEP[dtype], ("dgate", n, d))
