@@ -307,6 +307,14 @@ int check_status_word(fr_ctx* ctx)
     return FR_OK;
 }
 
+int lost_waits(fr_ctx* ctx)
+{
+    volatile unsigned* s = ctx->host_status;
+    if (!s || s[1] == 0) return FR_OK;
+    s[1] = 0;
+    return set_err(ctx, FR_HIP_ERROR, "a wait between workgroups ran out in an operator launched before; its results are NaN from there on");
+}
+
 void drain_stale_status(fr_ctx* ctx)
 {
     if (!ctx->persistent_pending) return;
@@ -401,6 +409,7 @@ int fr_ctx_create(fr_ctx** out, int device)
     ctx->device = device;
     ctx->num_cus = prop.multiProcessorCount > 0 ? prop.multiProcessorCount : 256;
     if (const char* e = getenv("FRIEDRICH_AMD_TEST_FORCE_SOLVE_TIMEOUT")) ctx->test_force_timeout = e[0] == '1';
+    if (const char* e = getenv("FRIEDRICH_AMD_TEST_WAIT_POLLS")) ctx->test_wait_polls = atoi(e);
     if (const char* e = getenv("FRIEDRICH_AMD_TEST_MAX_WORKGROUPS")) ctx->test_max_wgs = atoi(e);
     if (const char* e = getenv("FRIEDRICH_AMD_SMALL_TILES")) ctx->small_tiles = atoi(e);
     if (const char* e = getenv("FRIEDRICH_AMD_TEST_COMM_HANG")) {  // "schedule,rank,nth": see comm.hip (test hook)
@@ -439,7 +448,8 @@ int fr_ctx_create(fr_ctx** out, int device)
     }
     if (hipMalloc((void**)&ctx->xcc_word, 64) != hipSuccess || hipMemset(ctx->xcc_word, 0, 64) != hipSuccess ||
         hipMalloc((void**)&ctx->claim_ring, sizeof(unsigned) * 2 * kClaimSlots) != hipSuccess ||
-        hipMalloc((void**)&ctx->dyn_ring, sizeof(unsigned) * 2 * 256) != hipSuccess) {
+        hipMalloc((void**)&ctx->dyn_ring, sizeof(unsigned) * 2 * 256) != hipSuccess ||
+        ensure_status_word(ctx) != FR_OK) {  // (here: a captured call could not allocate it)
         fr_ctx_destroy(ctx);
         return FR_HIP_ERROR;
     }
@@ -510,7 +520,8 @@ int fr_ctx_synchronize(fr_ctx* ctx)
     if (!ctx) return FR_INVALID_ARGUMENT;
     FR_LOCK(ctx);
     FR_HIP(ctx, hipStreamSynchronize(ctx->stream));
-    return check_status_word(ctx);
+    FR_TRY(check_status_word(ctx));
+    return lost_waits(ctx);
 }
 
 const char* fr_last_error(const fr_ctx* ctx) { return ctx ? ctx->err.c_str() : "null context"; }

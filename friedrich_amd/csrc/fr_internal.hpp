@@ -150,7 +150,8 @@ struct fr_ctx {
     int64_t claim_next = 0;
     bool refine_now = false;      // state of the running operation (set under the context lock)
     double* cur_cest = nullptr;   // where the diagonal-block kernel of the running factorisation puts its estimates
-    // device-side waits report a timeout here (host-mapped, so the host can read it after any synchronisation)
+    // device-side waits report a timeout here (host-mapped, so the host can read it after any synchronisation): [0] those of the persistent
+    // solves and panels, [1] those inside an operator's launch (lost_waits)
     unsigned* host_status = nullptr;
     unsigned* dev_status = nullptr;
     bool solve_timeout_seen = false;  // a persistent solve timed out on this context: the entry point re-runs on the recursive path
@@ -158,6 +159,7 @@ struct fr_ctx {
     int64_t solve_retries = 0;        // how often that happened (fr_ctx_get_counter)
     int64_t stale_status_drops = 0;   // time-outs left behind by an entry point that returned early, dropped by the next one (drain_stale_status)
     int test_max_wgs = 0;             // FRIEDRICH_AMD_TEST_MAX_WORKGROUPS at context creation: cap on the grid of the persistent solves (tests: many blocks per workgroup)
+    int test_wait_polls = -1;         // FRIEDRICH_AMD_TEST_WAIT_POLLS at context creation: looks that a wait inside an operator's launch takes before it is lost (-1: as many as it likes)
     bool test_force_timeout = false;  // FRIEDRICH_AMD_TEST_FORCE_SOLVE_TIMEOUT=1 at context creation: every persistent solve reports a timeout (tests of the retry)
     int num_cus = 256;
     // hand-off granules of the persistent solves (grow-only)
@@ -447,6 +449,8 @@ int ensure_status_word(fr_ctx* ctx);
 int launch_trsm_narrow(fr_ctx* ctx, const fr_chol* c, double* B, int64_t m, int64_t ldb, bool fwd, int prof_cls);
 // FR_HIP_ERROR if a device-side wait timed out since the last check (call after a synchronisation)
 int check_status_word(fr_ctx* ctx);
+// FR_HIP_ERROR, once, if a wait inside an operator's launch (typed.hpp) has been lost since the last look
+int lost_waits(fr_ctx* ctx);
 // An entry point that launched a persistent solve and then left early (out of memory, bad argument) never read the status
 // word: the flag -- and a possible time-out -- would be reported by the NEXT, unrelated check (a factorisation would return a
 // spurious FR_HIP_ERROR).  Called at the start of solve_retry and of the factorisation entry points: waits for the stream,

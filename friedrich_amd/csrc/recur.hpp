@@ -36,6 +36,8 @@ struct RecArgs {
     int sum_lanes;             // ... lanes whose channels share a gate (0: every channel stores its part)
     int64_t part_r, part_c;
     void *ticket, *maps, *carry, *part;
+    unsigned* lost;  // host-visible: not 0 after a wait that ran out
+    int polls;       // looks that a wait takes before it does
 };
 
 // first row of sequence s, kept inside [0, n] whatever the caller's offsets say
@@ -179,7 +181,10 @@ __device__ __forceinline__ bool get_state(const unsigned long long* p, float& v)
     v = __uint_as_float((unsigned)w);
     return w != kUnset;
 }
-constexpr int kPolls = 1 << 22;  // (a bound that a running chip never meets: a wait that met it would leave NaN, not hang)
+// A bound that a running chip never meets.  A wait that does leaves NaN in its results and raises the context's word for lost waits, which the
+// host reads when it next waits or calls (lost_waits).
+constexpr int kPolls = 1 << 22;
+__device__ __forceinline__ void raise_lost(const RecArgs& a) { __hip_atomic_store(a.lost, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM); }
 
 // the workgroup's tile and channel group: in order of arrival where tiles wait for one another
 __device__ __forceinline__ unsigned claim_tile(const RecArgs& a, unsigned* slot)
@@ -510,7 +515,7 @@ __global__ __launch_bounds__(512) void rec_rows_kernel(const RecArgs a)
                                 const int64_t at = from + (k0 + k < ahead ? k0 + k : k0);
                                 ok = published(words + (at * a.d + ch) * kMapWords<S>, seen[k]) && ok;
                             }
-                            lost |= poll == kPolls;
+                            lost |= poll == a.polls;
                             if (ok || lost) break;
                             __builtin_amdgcn_s_sleep(1);
                         }
@@ -518,11 +523,15 @@ __global__ __launch_bounds__(512) void rec_rows_kernel(const RecArgs a)
                         for (int k = 0; k < 8; ++k)
                             if (k0 + k < ahead) sum = join(sum, seen[k]);
                     }
-                    if (lost) sum = {S(1), S(NAN), true};
+                    if (lost) {
+                        sum = {S(1), S(NAN), true};
+                        raise_lost(a);
+                    }
                     for (int poll = 0; block > 0; ++poll) {
                         if (get_state(states + (block - 1) * a.d + ch, st)) break;
-                        if (poll == kPolls) {
+                        if (poll == a.polls) {
                             st = S(NAN);
+                            raise_lost(a);
                             break;
                         }
                     }
@@ -854,12 +863,15 @@ __global__ __launch_bounds__(512) void rec_columns_kernel(const RecArgs a)
             bool lost = false;
             for (int poll = 0;; ++poll) {
                 const bool ok = lane >= ahead || published(words + (from + lane) * kMapWords<S>, m);
-                lost = poll == kPolls;
+                lost = poll == a.polls;
                 if (__all(ok) || lost) break;
                 __builtin_amdgcn_s_sleep(2);
             }
             if (lane >= ahead) m = {S(1), S(0), false};
-            if (lost) m = {S(1), S(NAN), true};
+            if (lost) {
+                m = {S(1), S(NAN), true};
+                if (lane == 0) raise_lost(a);
+            }
 #pragma unroll
             for (int d = 1; d < 64; d *= 2) {
                 const Map<S> p = shift_up(m, d);
@@ -869,8 +881,9 @@ __global__ __launch_bounds__(512) void rec_columns_kernel(const RecArgs a)
             const Map<S> through = join(m, all);
             for (int poll = 0; window > 0; ++poll) {
                 if (get_state(states + window - 1, st)) break;
-                if (poll == kPolls) {
+                if (poll == a.polls) {
                     st = S(NAN);
+                    if (lane == 0) raise_lost(a);
                     break;
                 }
                 __builtin_amdgcn_s_sleep(1);
@@ -1043,6 +1056,7 @@ static int rec_prepare(fr_ctx* ctx, RecArgs& a, int64_t rows, int64_t stretches_
     const int64_t words = a.tiles > 1 ? 1 + maps + states : 0;
     if (words + parts == 0) return FR_OK;
     FR_TRY(ws.get((size_t)(words * 8 + parts * (int64_t)sizeof(S))));
+    a.lost = ctx->dev_status + 1, a.polls = ctx->test_wait_polls >= 0 ? ctx->test_wait_polls : kPolls;
     unsigned long long* p = (unsigned long long*)ws.p;
     a.ticket = p;
     a.maps = p + 1;

@@ -89,7 +89,7 @@ int Operand::commit()
     if (!host) return FR_OK;
     FR_HIP(ctx, hipMemcpy2DAsync(host, (size_t)(host_ld * elem_), dev, (size_t)(line_ * elem_), (size_t)(line_ * elem_), (size_t)lines_, hipMemcpyDeviceToHost, ctx->stream));
     FR_HIP(ctx, hipStreamSynchronize(ctx->stream));
-    return FR_OK;
+    return lost_waits(ctx);
 }
 
 }  // namespace fr

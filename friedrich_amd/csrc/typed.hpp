@@ -156,6 +156,7 @@ int op_entry(fr_ctx* ctx, F&& body)
         FR_LOCK(ctx);
         DeviceScope dev;
         FR_TRY(dev.enter(ctx));
+        FR_TRY(lost_waits(ctx));  // (of an earlier call whose results stayed on the device)
         return body();
     } catch (const std::bad_alloc&) {
         return FR_OUT_OF_MEMORY;

@@ -171,6 +171,7 @@ int fr_ctx_set_option(fr_ctx* ctx, const char* name, int64_t value);
  *   FRIEDRICH_AMD_SMALL_TILES       A/B override of the 32-row-tile rule (gemm_f64.hip)
  *   FRIEDRICH_AMD_LOCAL_SYNC = 1    in-process transport: synchronise around every collective instead of ordering by events
  *   test hooks: FRIEDRICH_AMD_TEST_MAX_WORKGROUPS (cap on the grid of the persistent solves: many blocks per workgroup),
+ *   FRIEDRICH_AMD_TEST_WAIT_POLLS (looks that a wait inside an operator's launch takes before it is lost; 0: every one is),
  *   FRIEDRICH_AMD_TEST_FORCE_SOLVE_TIMEOUT = 1 (every persistent solve reports a time-out: the retry path),
  *   FRIEDRICH_AMD_TEST_COMM_HANG = "schedule,rank,nth" (that rank skips its nth collective under that schedule: the watchdog). */
 int fr_ctx_get_counter(fr_ctx* ctx, const char* name, int64_t* out);
@@ -361,6 +362,9 @@ int fr_grad_terms(fr_chol* chol, const fr_kprog* kernel, const double* y, double
  *    A capture keeps its workspace until the context is destroyed, and takes it from what eager calls left in the context's pool:
  *    run the calls once before each capture (FR_OUT_OF_MEMORY otherwise).  Host data in a captured call is refused.  Graphs of one
  *    context may be replayed side by side, one graph not beside itself.
+ *  - on device data a call returns before its work is done.  The launches that pass results between workgroups bound their waits: one that
+ *    runs out, which a running GPU does not come to, leaves NaN, and fr_ctx_synchronize or the next of these calls returns FR_HIP_ERROR,
+ *    once (on host data the call itself).
  *  - an output must not overlap an input or another output, except where a call says so. */
 typedef enum { FR_F64 = 0, FR_F32 = 1, FR_BF16 = 2, FR_F16 = 3 } fr_dtype;
 

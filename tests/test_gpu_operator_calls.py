@@ -1,0 +1,49 @@
+"""What surrounds the operators past the cube: lost waits, workspaces, streams."""
+import numpy as np
+import pytest
+
+from test_gpu_recurrence import host, problem, put, tctx, torch_types  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("layout,n,d", [("col", 60000, 2), ("row", 6000, 130)])
+def test_a_lost_wait_is_an_error(monkeypatch, layout, n, d):
+    """FRIEDRICH_AMD_TEST_WAIT_POLLS = 0: every tile that waits for others gives up at its first look.  The results are NaN, the kernels end as
+    ever, and the call that waits for them says so -- the next one where the results stay on the device"""
+    import torch
+    from friedrich_amd import _capi as C
+    from friedrich_amd.device import Context, FriedrichError
+
+    rng = np.random.default_rng(63)
+    gate, x, h0, _ = problem(rng, n, d, d, 1, "log", "f32", layout)
+    monkeypatch.setenv("FRIEDRICH_AMD_TEST_WAIT_POLLS", "0")
+    c = Context()
+    monkeypatch.delenv("FRIEDRICH_AMD_TEST_WAIT_POLLS")
+    c.set_stream(torch.cuda.current_stream().cuda_stream)
+    h, last = c.recurrence(gate, x, h0=h0)
+    with pytest.raises(FriedrichError) as e:
+        c.synchronize()
+    assert e.value.status == C.FR_HIP_ERROR and torch.isnan(last).any()
+    c.synchronize()  # (said once)
+    c.recurrence(gate, x, h0=h0)
+    torch.cuda.synchronize()
+    with pytest.raises(FriedrichError) as e:  # the next operator's call
+        c.route(torch.zeros(4, 4, device="cuda"), 1)
+    assert e.value.status == C.FR_HIP_ERROR
+    got, _ = c.route(torch.zeros(4, 4, device="cuda"), 1)
+    assert (got == 0).all()
+    with pytest.raises(FriedrichError) as e:  # host data: the call itself
+        c.recurrence(*(np.array(host(t), dtype=np.float32, order="C" if layout == "row" else "F") for t in (gate, x)))
+    assert e.value.status == C.FR_HIP_ERROR
+    # calls whose rows lie in one tile (8 waves of 4 rows are the smallest) do not wait; a factorisation does not see the operators' word
+    short = tuple(t[:32] for t in (gate, x))
+    c.recurrence(*short)
+    c.recurrence(gate, x, h0=h0)
+    A = np.asfortranarray(rng.random((300, 3)))
+    chol = c.cholesky_from_inputs(("squared_exp", 1.0, 1.0), A, 0.1)
+    assert np.isfinite(chol.solve(np.ones(300))).all()
+    chol.free()
+    with pytest.raises(FriedrichError):
+        c.synchronize()
+    c.close()
