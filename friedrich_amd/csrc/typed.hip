@@ -47,7 +47,8 @@ int OpWorkspace::get(size_t bytes)
     DevBuf* best = nullptr;
     for (DevBuf& b : ctx->pool)
         if (b.p && !b.in_use && b.cap >= bytes && (!best || b.cap < best->cap)) best = &b;
-    if (!best)
+    // (kept for good: of about the size asked for, as an eager call takes and leaves one -- ws_get)
+    if (!best || best->cap > bytes * 2 + (1u << 20))
         return set_err(ctx, FR_OUT_OF_MEMORY,
                        "a captured call needs a workspace of %zu bytes and cannot allocate it: run the calls once outside the capture before each capture", bytes);
     ctx->captured.push_back({best->p, best->cap, id, ctx->stream, true});

@@ -47,3 +47,45 @@ def test_a_lost_wait_is_an_error(monkeypatch, layout, n, d):
     with pytest.raises(FriedrichError):
         c.synchronize()
     c.close()
+
+
+def test_a_capture_leaves_buffers_of_other_sizes():
+    """a captured call keeps its workspace for good: it takes one of about its size, not whatever is free"""
+    import torch
+    from friedrich_amd.device import Context, FriedrichError
+
+    rng = np.random.default_rng(61)
+    c, side = Context(), torch.cuda.Stream()
+    gate, x, h0, _ = problem(rng, 9000, 2, 2, 1, "log", "f64", "col")
+    out, last = torch.zeros_like(x), torch.zeros_like(h0)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        c.set_stream(side.cuda_stream)
+        A = np.asfortranarray(rng.random((3000, 200)))
+        want = c.gram(("squared_exp", 1.0, 1.0), A, A)  # leaves buffers of 5 and 72 MB
+        held = c.counter("pool_bytes")
+        assert held > 70 << 20
+        g = torch.cuda.CUDAGraph()
+        refused = None
+        with torch.cuda.graph(g, stream=side):
+            try:
+                c.recurrence(gate, x, h0=h0, out=out, last=last)
+            except FriedrichError as e:
+                refused = str(e)
+        assert refused and "once outside" in refused
+        c.recurrence(gate, x, h0=h0, out=out, last=last)
+        side.synchronize()
+        eager = out.clone()
+        g2 = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g2, stream=side):
+            c.recurrence(gate, x, h0=h0, out=out, last=last)
+        for _ in range(3):
+            out.zero_()
+            g2.replay()
+            side.synchronize()
+            assert torch.equal(out, eager)
+            assert np.array_equal(c.gram(("squared_exp", 1.0, 1.0), A, A), want)
+        assert c.counter("pool_bytes") <= held + (2 << 20)  # (the large ones are free for calls of their size)
+    torch.cuda.synchronize()
+    del g, g2
+    c.close()
