@@ -520,7 +520,7 @@ static int64_t piece_rows(int64_t want, int64_t tiles, int64_t rows, int64_t exp
 {
     const int64_t pieces = (want + tiles - 1) / tiles, each = rows / experts + 1;
     int64_t piece = (each + pieces - 1) / pieces;
-    const int64_t bound = lanes * (rows >> 10) >> 15;
+    const int64_t bound = lanes * rows >> 25;
     return round_up(piece > bound ? piece : bound, least);
 }
 

@@ -89,3 +89,31 @@ def test_a_capture_leaves_buffers_of_other_sizes():
     torch.cuda.synchronize()
     del g, g2
     c.close()
+
+
+def test_workspace_of_many_slots_and_few_points(tctx):  # noqa: F811
+    """sums of pieces take about 256 MB at most, however many slots there are to an expert's few points"""
+    import torch
+    from friedrich_amd.device import Context
+
+    rng = np.random.default_rng(62)
+    c = Context()
+    c.set_stream(torch.cuda.current_stream().cuda_stream)
+    n, experts, m, k = 1000, 64, 1 << 19, 2
+    X = put(rng.random((n, 1)), "col", torch.float64)
+    Xq = put(rng.random((m, 1)), "col", torch.float64)
+    offsets = torch.arange(experts + 1, device="cuda") * n // experts
+    chosen = torch.randint(0, experts, (k, m), device="cuda", dtype=torch.int32).t()
+    w = torch.rand(k, m, device="cuda", dtype=torch.float64).t()
+    alpha = torch.randn(n, device="cuda", dtype=torch.float64)
+    before = c.counter("pool_bytes")
+    mean, slots = c.experts_predict(("squared_exp", 0.3, 1.0), X, alpha, offsets, Xq, chosen, w)
+    own = 8 * m * k * (1 + 1 + 2)  # (query points packed, list and places, two pieces more than the bound)
+    assert c.counter("pool_bytes") - before <= (256 << 20) + own + (4 << 20)
+    # a sample against the definition: 16 points an expert and the exponential, 40 roundings in all at most
+    for q in range(0, m, m // 50):
+        for j in range(k):
+            lo, hi = int(offsets[chosen[q, j]]), int(offsets[chosen[q, j] + 1])
+            kx = torch.exp(-((X[lo:hi, 0] - Xq[q, 0]) ** 2) / (2 * 0.3 ** 2))
+            assert abs(float(slots[q, j] - (kx * alpha[lo:hi]).sum())) <= 40 * 2.0**-52 * float((kx * alpha[lo:hi].abs()).sum())
+    c.close()
