@@ -572,6 +572,7 @@ static int experts_check(fr_ctx* ctx, const fr_kprog* kernel, int64_t n, int64_t
 {
     FR_TRY(kprog_check(ctx, kernel));
     if (n < 0 || d < 1 || m < 0) return set_err(ctx, FR_SHAPE, "%lld points of %lld features, %lld queries", (long long)n, (long long)d, (long long)m);
+    if (d > (int64_t)1 << 24) return set_err(ctx, FR_SHAPE, "%lld features: at most 2^24", (long long)d);  // (the kernels count a block's bytes in 32 bits)
     if (n_experts < 1 || n_experts > kMaxExperts) return set_err(ctx, FR_SHAPE, "%lld experts: 1 to %d", (long long)n_experts, kMaxExperts);
     if (k < 1 || k > 64) return set_err(ctx, FR_SHAPE, "%lld slots a query: 1 to 64", (long long)k);
     if (m > ((int64_t)1 << 30) / k || n > (int64_t)1 << 31) return set_err(ctx, FR_SHAPE, "more than 2^30 slots or 2^31 points");

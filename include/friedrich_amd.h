@@ -419,7 +419,7 @@ int fr_route_backward(fr_ctx* ctx, int dtype, int layout, int score, int64_t n, 
                       const void* experts, int64_t lde, int64_t k, int renormalise, double scale, const void* dweights, int64_t lddw,
                       void* dlogits, int64_t lddl);
 /* Means of m query points from n_experts <= 1024 local models that share a kernel program (f64, column-major like the predict
- * family).  X (n x d) and alpha (n values: each expert's own K^-1 y) hold the experts' points one expert after the other, expert e has the rows
+ * family).  X (n x d, d <= 2^24) and alpha (n values: each expert's own K^-1 y) hold the experts' points one expert after the other, expert e has the rows
  * [offsets[e], offsets[e + 1]) (offsets: n_experts + 1 int64, as in fr_recurrence).  experts (m x k int32), weights (m x k): what
  * fr_route gives, k <= 64; slots outside [0, n_experts) have a mean of 0.
  *   out_slots[q, j] = sum_i k(x_q, x_i) alpha_i over the points of experts[q, j]    (m x k; may be NULL)

@@ -117,3 +117,21 @@ def test_workspace_of_many_slots_and_few_points(tctx):  # noqa: F811
             kx = torch.exp(-((X[lo:hi, 0] - Xq[q, 0]) ** 2) / (2 * 0.3 ** 2))
             assert abs(float(slots[q, j] - (kx * alpha[lo:hi]).sum())) <= 40 * 2.0**-52 * float((kx * alpha[lo:hi].abs()).sum())
     c.close()
+
+
+def test_more_features_than_an_index_holds(tctx):  # noqa: F811
+    """refused before anything is read"""
+    import ctypes
+
+    import torch
+    from friedrich_amd import _capi as C
+
+    z = torch.zeros(8, dtype=torch.float64, device="cuda")
+    off = np.array([0, 1], dtype=np.int64)
+    p, e = C.kprog(("squared_exp", 1.0, 1.0)), torch.zeros(1, dtype=torch.int32, device="cuda")
+    at = z.data_ptr()
+    d = (1 << 24) + 1
+    st = tctx.lib.fr_experts_predict(tctx.h, ctypes.byref(p), at, 1, 1, d, at, off.ctypes.data, 1, at, 1, 1, e.data_ptr(), 1, at, 1, 1, None, at, None, 0)
+    assert st == C.FR_SHAPE
+    st = tctx.lib.fr_experts_backward(tctx.h, ctypes.byref(p), at, 1, 1, d, off.ctypes.data, 1, at, 1, 1, e.data_ptr(), 1, at, 1, 1, at, 1, at, at, 1, at)
+    assert st == C.FR_SHAPE
