@@ -238,6 +238,8 @@ def _line(t, length, name):
 class Context:
     """fr_ctx: one per (process, GPU).  Fails loudly when no gfx950 device / library is present."""
 
+    _given = False  # whether set_stream has named the stream to work on
+
     def __init__(self, device=-1):
         self.lib = C.load()
         h = ctypes.c_void_p()
@@ -266,7 +268,24 @@ class Context:
         return st
 
     def set_stream(self, hip_stream_ptr):
+        """work on this stream from here on (torch.cuda.current_stream().cuda_stream): calls on tensors take their turn among torch's work there"""
         self.check(self.lib.fr_ctx_set_stream(self.h, ctypes.c_void_p(hip_stream_ptr)))
+        self._given = True
+
+    def _in_turn(self, *tensors):
+        """Before a launch on tensors: torch's work on them is done, if the context works on a stream of its own.  -> whether torch's work has to
+        wait for the call in turn"""
+        if self._given:
+            return False
+        for t in tensors:
+            if t is not None and _is_torch(t) and t.is_cuda:
+                import torch
+
+                if torch.cuda.is_current_stream_capturing():
+                    raise ValueError("a call on the context's own stream cannot be captured: set_stream first")
+                torch.cuda.current_stream(t.device).synchronize()
+                return True
+        return False
 
     def set_option(self, name, value):
         self.check(self.lib.fr_ctx_set_option(self.h, name.encode(), int(value)))
@@ -436,8 +455,8 @@ class Context:
                                              ctypes.byref(h)))
         return Cholesky(self, h)
 
-    # (the calls from here on take torch tensors and numpy arrays.  With torch tensors set_stream the stream that torch works on first: the
-    # context's own stream does not wait for it.)
+    # The calls from here on take torch tensors and numpy arrays.  After set_stream they are launched on that stream and do not wait; on the
+    # context's own stream, a call on tensors waits for torch's current stream before and for its own work after.
     # ordered inputs: the gated linear recurrence -------------------------------------------------------
     def recurrence(self, gate, x, form="log", offsets=None, h0=None, out=None, last=None):
         """h_t = a_t h_{t-1} + c_t x_t over packed sequences (fr_recurrence).  gate: n x gate_cols, x: n x d, torch tensors or numpy arrays
@@ -455,8 +474,11 @@ class Context:
         _typed(gate, x.dtype, "gate"), _typed(h0, wide, "h0"), _typed(out, x.dtype, "out"), _typed(last, wide, "last"), _ints(offsets, 8, "offsets")
         g, xx, s, h, e = (_lead(gate, layout, (n, cols), "gate"), _lead(x, layout, (n, d), "x"), _lead(h0, layout, (nseq, d), "h0"),
                           _lead(out, layout, (n, d), "out"), _lead(last, layout, (nseq, d), "last"))
-        self.check(self.lib.fr_recurrence(self.h, _code(x), layout, C.GATE_FORMS[form], n, d, g[0], cols, g[1], xx[0], xx[1],
-                                          _line(offsets, nseq + 1, "offsets"), nseq, s[0], s[1], h[0], h[1], e[0], e[1]))
+        form, code, cuts = C.GATE_FORMS[form], _code(x), _line(offsets, nseq + 1, "offsets")
+        wait = self._in_turn(gate, x, offsets, h0, out, last)
+        self.check(self.lib.fr_recurrence(self.h, code, layout, form, n, d, g[0], cols, g[1], xx[0], xx[1], cuts, nseq, s[0], s[1], h[0], h[1], e[0], e[1]))
+        if wait:
+            self.synchronize()
         return out, last
 
     def recurrence_backward(self, gate, x, h, dh, form="log", offsets=None, h0=None, dlast=None, dgate=None, dx=None, dh0=None):
@@ -483,9 +505,12 @@ class Context:
         g, xx, s, hh, y, e = (_lead(gate, layout, (n, cols), "gate"), _lead(x, layout, big, "x"), _lead(h0, layout, small, "h0"), _lead(h, layout, big, "h"),
                               _lead(dh, layout, big, "dh"), _lead(dlast, layout, small, "dlast"))
         dg, du, ds = _lead(dgate, layout, (n, cols), "dgate"), _lead(dx, layout, big, "dx"), _lead(dh0, layout, small, "dh0")
-        self.check(self.lib.fr_recurrence_backward(self.h, _code(dh), layout, C.GATE_FORMS[form], n, d, g[0], cols, g[1], xx[0], xx[1],
-                                                   _line(offsets, nseq + 1, "offsets"), nseq, s[0], s[1], hh[0], hh[1], y[0], y[1], e[0], e[1], dg[0], dg[1],
-                                                   du[0], du[1], ds[0], ds[1]))
+        form, code, cuts = C.GATE_FORMS[form], _code(dh), _line(offsets, nseq + 1, "offsets")
+        wait = self._in_turn(gate, x, h, dh, offsets, h0, dlast, dgate, dx, dh0)
+        self.check(self.lib.fr_recurrence_backward(self.h, code, layout, form, n, d, g[0], cols, g[1], xx[0], xx[1], cuts, nseq, s[0], s[1], hh[0], hh[1],
+                                                   y[0], y[1], e[0], e[1], dg[0], dg[1], du[0], du[1], ds[0], ds[1]))
+        if wait:
+            self.synchronize()
         return dgate, dx, dh0
 
     def markov_product(self, kernel, t, V, noise=0.0, out=None):
@@ -500,7 +525,10 @@ class Context:
         o = _Mat(out, writable=True)
         if (o.rows, o.cols) != (v.rows, v.cols):
             raise FriedrichError(C.FR_SHAPE, "out has another shape than V")
+        wait = self._in_turn(t, V, out)
         self.check(self.lib.fr_markov_product(self.h, ctypes.byref(p), tp, v.rows, v.ptr, v.cols, v.ld, float(noise), o.ptr, o.ld))
+        if wait:
+            self.synchronize()
         return out
 
     # local experts: the router and their product -----------------------------------------------------------
@@ -517,9 +545,12 @@ class Context:
         if bias is not None and _code(bias) != C.FR_F64:
             raise ValueError("bias: float64 is needed")
         z, at, w = _lead(logits, layout, (n, e), "logits"), _lead(experts, layout, (n, k), "experts"), _lead(weights, layout, (n, k), "weights")
-        self.check(self.lib.fr_route(self.h, _code(logits), layout, C.SCORES[score], n, e, z[0], z[1], _line(bias, e, "bias"), groups,
-                                     groups if top_groups is None else top_groups, k, 1 if renormalise else 0, float(scale), at[0], at[1], w[0], w[1],
-                                     _line(counts, e, "counts")))
+        code, score, b, seen = _code(logits), C.SCORES[score], _line(bias, e, "bias"), _line(counts, e, "counts")
+        wait = self._in_turn(logits, bias, experts, weights, counts)
+        self.check(self.lib.fr_route(self.h, code, layout, score, n, e, z[0], z[1], b, groups, groups if top_groups is None else top_groups, k,
+                                     1 if renormalise else 0, float(scale), at[0], at[1], w[0], w[1], seen))
+        if wait:
+            self.synchronize()
         return experts, weights
 
     def route_backward(self, logits, experts, dweights, score="softmax", renormalise=True, scale=1.0, dlogits=None):
@@ -531,8 +562,12 @@ class Context:
         _ints(experts, 4, "experts"), _typed(dweights, _wide(logits), "dweights"), _typed(dlogits, logits.dtype, "dlogits")
         z, at, w, o = (_lead(logits, layout, (n, e), "logits"), _lead(experts, layout, (n, k), "experts"), _lead(dweights, layout, (n, k), "dweights"),
                        _lead(dlogits, layout, (n, e), "dlogits"))
-        self.check(self.lib.fr_route_backward(self.h, _code(logits), layout, C.SCORES[score], n, e, z[0], z[1], at[0], at[1], k, 1 if renormalise else 0,
-                                              float(scale), w[0], w[1], o[0], o[1]))
+        code, score = _code(logits), C.SCORES[score]
+        wait = self._in_turn(logits, experts, dweights, dlogits)
+        self.check(self.lib.fr_route_backward(self.h, code, layout, score, n, e, z[0], z[1], at[0], at[1], k, 1 if renormalise else 0, float(scale), w[0], w[1],
+                                              o[0], o[1]))
+        if wait:
+            self.synchronize()
         return dlogits
 
     def experts_predict(self, kernel, X, alpha, offsets, Xq, experts, weights, prior_q=None, out=None, slots=None):
@@ -549,8 +584,11 @@ class Context:
         _ints(experts, 4, "experts"), _ints(offsets, 8, "offsets")
         x, q, at, w, s = (_lead(X, col, (n, d), "X"), _lead(Xq, col, (m, d), "Xq"), _lead(experts, col, (m, k), "experts"), _lead(weights, col, (m, k), "weights"),
                           _lead(slots, col, (m, k), "slots"))
-        self.check(self.lib.fr_experts_predict(self.h, ctypes.byref(p), x[0], n, x[1], d, _line(alpha, n, "alpha"), _line(offsets, e + 1, "offsets"), e, q[0], m, q[1],
-                                               at[0], at[1], w[0], w[1], k, _line(prior_q, m, "prior_q"), _line(out, m, "out"), s[0], s[1]))
+        al, cuts, prior, o = _line(alpha, n, "alpha"), _line(offsets, e + 1, "offsets"), _line(prior_q, m, "prior_q"), _line(out, m, "out")
+        wait = self._in_turn(X, alpha, offsets, Xq, experts, weights, prior_q, out, slots)
+        self.check(self.lib.fr_experts_predict(self.h, ctypes.byref(p), x[0], n, x[1], d, al, cuts, e, q[0], m, q[1], at[0], at[1], w[0], w[1], k, prior, o, s[0], s[1]))
+        if wait:
+            self.synchronize()
         return out, slots
 
     def experts_backward(self, kernel, X, offsets, Xq, experts, weights, slots, dmean, dweights=None, dalpha=None):
@@ -567,8 +605,12 @@ class Context:
         _ints(experts, 4, "experts"), _ints(offsets, 8, "offsets")
         x, q, at, w, s, dw = (_lead(X, col, (n, d), "X"), _lead(Xq, col, (m, d), "Xq"), _lead(experts, col, (m, k), "experts"), _lead(weights, col, (m, k), "weights"),
                               _lead(slots, col, (m, k), "slots"), _lead(dweights, col, (m, k), "dweights"))
-        self.check(self.lib.fr_experts_backward(self.h, ctypes.byref(p), x[0], n, x[1], d, _line(offsets, e + 1, "offsets"), e, q[0], m, q[1], at[0], at[1], w[0], w[1], k,
-                                                s[0], s[1], _line(dmean, m, "dmean"), dw[0], dw[1], _line(dalpha, n, "dalpha")))
+        cuts, dm, da = _line(offsets, e + 1, "offsets"), _line(dmean, m, "dmean"), _line(dalpha, n, "dalpha")
+        wait = self._in_turn(X, offsets, Xq, experts, weights, slots, dmean, dweights, dalpha)
+        self.check(self.lib.fr_experts_backward(self.h, ctypes.byref(p), x[0], n, x[1], d, cuts, e, q[0], m, q[1], at[0], at[1], w[0], w[1], k, s[0], s[1], dm,
+                                                dw[0], dw[1], da))
+        if wait:
+            self.synchronize()
         return dweights, dalpha
 
 

@@ -135,3 +135,39 @@ def test_more_features_than_an_index_holds(tctx):  # noqa: F811
     assert st == C.FR_SHAPE
     st = tctx.lib.fr_experts_backward(tctx.h, ctypes.byref(p), at, 1, 1, d, off.ctypes.data, 1, at, 1, 1, e.data_ptr(), 1, at, 1, 1, at, 1, at, at, 1, at)
     assert st == C.FR_SHAPE
+
+
+def test_a_context_on_its_own_stream():
+    """without set_stream: what torch has queued on its stream is there when the call reads it, and what the call wrote when torch does"""
+    import torch
+    from friedrich_amd.device import Context
+
+    rng = np.random.default_rng(64)
+    c = Context()
+    gate, x, h0, _ = problem(rng, 20000, 3, 3, 4, "log", "f64", "row")
+    offsets = torch.tensor([0, 100, 5000, 12000, 19000], dtype=torch.int64, device="cuda")
+    z = put(rng.standard_normal((3000, 16)), "row", torch.float32)
+    torch.cuda.synchronize()
+    ref = Context()
+    ref.set_stream(torch.cuda.current_stream().cuda_stream)
+    want = ref.recurrence(gate, x, offsets=offsets, h0=h0)
+    want_g = ref.recurrence_backward(gate, x, want[0], x, offsets=offsets, h0=h0)
+    want_r = ref.route(z, 2)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        x2, z2 = torch.zeros_like(x), torch.zeros_like(z)
+        torch.cuda._sleep(20_000_000)  # (clock ticks of a kernel that ends by itself: torch's stream is late)
+        x2.copy_(x)
+        z2.copy_(z)
+        h, last = c.recurrence(gate, x2, offsets=offsets, h0=h0)
+        h2, last2 = h + 0, last + 0
+        assert torch.equal(h2, want[0]) and torch.equal(last2, want[1])
+        torch.cuda._sleep(20_000_000)
+        y = torch.zeros_like(x)
+        y.copy_(x)
+        got = c.recurrence_backward(gate, y, h, y, offsets=offsets, h0=h0)
+        assert all(torch.equal(a + 0, b) for a, b in zip(got, want_g))
+        e, w = c.route(z2, 2)
+        assert torch.equal(e + 0, want_r[0]) and torch.equal(w + 0, want_r[1])
+    c.close()
+    ref.close()

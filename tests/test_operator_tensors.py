@@ -1,0 +1,85 @@
+"""What the binding of the operators past the cube does around a call on torch tensors (no GPU: the library is replaced by a recorder, tensors
+in host memory say that they lie on the GPU)."""
+import numpy as np
+import pytest
+
+from friedrich_amd.device import Context
+from test_operator_arguments import Recorder
+
+torch = pytest.importorskip("torch")
+KERNEL = ("squared_exp", 1.0, 1.0)
+
+
+class OnGpu(torch.Tensor):
+    is_cuda = True
+
+
+def there(*shape, dtype=torch.float64):
+    return torch.zeros(shape, dtype=dtype).as_subclass(OnGpu)
+
+
+def columns(rows, cols, dtype=torch.float64):
+    return there(cols, rows, dtype=dtype).t()
+
+
+@pytest.fixture
+def ctx(monkeypatch):
+    c = Context.__new__(Context)
+    c.lib, c.h, c._children = Recorder(), 1, set()
+
+    class Stream:
+        def synchronize(self):
+            c.lib.calls.append(("torch waits", ()))
+
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    yield c
+    c.h = None
+
+
+def calls(c):
+    """one call of every operator on tensors"""
+    x, g, off = there(5, 4), there(5, 1), there(3, dtype=torch.int64)
+    X, Xq, e, w = columns(10, 3), columns(4, 3), columns(4, 2, torch.int32), columns(4, 2)
+    v = [there(n) for n in (10, 4)]
+    return {
+        "fr_recurrence": lambda: c.recurrence(g, x, offsets=off),
+        "fr_recurrence_backward": lambda: c.recurrence_backward(g, None, x, x, offsets=off),
+        "fr_markov_product": lambda: c.markov_product(("exponential", 1.0, 1.0), v[0], columns(10, 2)),
+        "fr_route": lambda: c.route(there(6, 8), 2),
+        "fr_route_backward": lambda: c.route_backward(columns(4, 8), e, w),
+        "fr_experts_predict": lambda: c.experts_predict(KERNEL, X, v[0], off, Xq, e, w),
+        "fr_experts_backward": lambda: c.experts_backward(KERNEL, X, off, Xq, e, w, w, v[1]),
+    }
+
+
+def test_turns_on_the_contexts_own_stream(ctx):
+    for name, call in calls(ctx).items():
+        ctx.lib.calls.clear()
+        call()
+        assert [n for n, _ in ctx.lib.calls] == ["torch waits", name, "fr_ctx_synchronize"], name
+
+
+def test_no_waits_on_a_stream_that_was_given(ctx):
+    ctx.set_stream(0)
+    for name, call in calls(ctx).items():
+        ctx.lib.calls.clear()
+        call()
+        assert [n for n, _ in ctx.lib.calls] == [name], name
+
+
+def test_no_waits_for_host_arrays(ctx):
+    ctx.recurrence(np.zeros((5, 1)), np.zeros((5, 4)))
+    ctx.route(np.zeros((6, 8)), 2)
+    assert [n for n, _ in ctx.lib.calls] == ["fr_recurrence", "fr_route"]
+
+
+def test_the_contexts_own_stream_cannot_be_captured(ctx, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for name, call in calls(ctx).items():
+        with pytest.raises(ValueError, match="set_stream"):
+            call()
+    assert not ctx.lib.calls
+    ctx.set_stream(0)
+    for call in calls(ctx).values():
+        call()
