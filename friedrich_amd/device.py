@@ -273,8 +273,14 @@ class Context:
         self._given = True
 
     def _in_turn(self, *tensors):
-        """Before a launch on tensors: torch's work on them is done, if the context works on a stream of its own.  -> whether torch's work has to
-        wait for the call in turn"""
+        """Before a launch on tensors: none of them expects to be differentiated through, and torch's work on them is done, if the context works on
+        a stream of its own.  -> whether torch's work has to wait for the call in turn"""
+        for t in tensors:
+            if getattr(t, "requires_grad", False):
+                import torch
+
+                if torch.is_grad_enabled():
+                    raise ValueError("autograd does not see through this call: detach() its tensors, and take the gradients from the operator's own backward pass")
         if self._given:
             return False
         for t in tensors:
@@ -455,7 +461,8 @@ class Context:
                                              ctypes.byref(h)))
         return Cholesky(self, h)
 
-    # The calls from here on take torch tensors and numpy arrays.  After set_stream they are launched on that stream and do not wait; on the
+    # The calls from here on take torch tensors and numpy arrays.  They are no part of an autograd graph: tensors that require gradients are
+    # refused outside torch.no_grad() and an autograd function's own passes.  After set_stream they are launched on that stream and do not wait; on the
     # context's own stream, a call on tensors waits for torch's current stream before and for its own work after.
     # ordered inputs: the gated linear recurrence -------------------------------------------------------
     def recurrence(self, gate, x, form="log", offsets=None, h0=None, out=None, last=None):

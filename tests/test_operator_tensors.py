@@ -83,3 +83,39 @@ def test_the_contexts_own_stream_cannot_be_captured(ctx, monkeypatch):
     ctx.set_stream(0)
     for call in calls(ctx).values():
         call()
+
+
+def test_gradients_are_not_lost_silently(ctx):
+    """a call on tensors that autograd follows would return results without a graph: refused, allowed where autograd is off"""
+    x, g = torch.zeros(5, 4, dtype=torch.float64, requires_grad=True), torch.zeros(5, 1, dtype=torch.float64)
+    z = torch.zeros(6, 8, requires_grad=True)
+    w = columns(4, 2).requires_grad_()
+    refused = [lambda: ctx.recurrence(g, x), lambda: ctx.recurrence(g, x.detach(), h0=torch.zeros(1, 4, dtype=torch.float64, requires_grad=True)),
+               lambda: ctx.recurrence_backward(g, None, x.detach(), x), lambda: ctx.route(z, 2),
+               lambda: ctx.markov_product(("exponential", 1.0, 1.0), there(10), columns(10, 2).requires_grad_()),
+               lambda: ctx.route_backward(columns(4, 8), columns(4, 2, torch.int32), w),
+               lambda: ctx.experts_predict(KERNEL, columns(10, 3), there(10), there(3, dtype=torch.int64), columns(4, 3), columns(4, 2, torch.int32), w),
+               lambda: ctx.experts_backward(KERNEL, columns(10, 3), there(3, dtype=torch.int64), columns(4, 3), columns(4, 2, torch.int32), w, columns(4, 2), there(4))]
+    for call in refused:
+        with pytest.raises(ValueError, match="autograd"):
+            call()
+    assert not ctx.lib.calls
+    with torch.no_grad():
+        for call in refused:
+            call()
+
+    class Paths(torch.autograd.Function):
+        @staticmethod
+        def forward(f, gate, x):
+            h, _ = ctx.recurrence(gate, x)
+            f.save_for_backward(gate, x, h)
+            return h
+
+        @staticmethod
+        def backward(f, dh):
+            gate, x, h = f.saved_tensors
+            return ctx.recurrence_backward(gate, x, h, dh.contiguous())[:2]
+
+    ctx.lib.calls.clear()
+    Paths.apply(g.detach().requires_grad_(), x).sum().backward()
+    assert [n for n, _ in ctx.lib.calls] == ["fr_recurrence", "fr_recurrence_backward"] and x.grad.shape == x.shape
