@@ -216,7 +216,10 @@ def _program(kernel):
     """C.kprog, kept for the specs a program calls with again and again"""
     if isinstance(kernel, C.KProg):
         return kernel
-    p = _programs.get(kernel)
+    try:
+        p = _programs.get(kernel)
+    except TypeError:  # a list is a spec like a tuple, and no key
+        return C.kprog(kernel)
     if p is None:
         if len(_programs) > 64:
             _programs.clear()

@@ -119,3 +119,15 @@ def test_gradients_are_not_lost_silently(ctx):
     ctx.lib.calls.clear()
     Paths.apply(g.detach().requires_grad_(), x).sum().backward()
     assert [n for n, _ in ctx.lib.calls] == ["fr_recurrence", "fr_recurrence_backward"] and x.grad.shape == x.shape
+
+
+def test_kernels_given_as_lists(ctx):
+    """a spec is a sequence, as for the other calls that take one: lists, lists within tuples, a program made before"""
+    from friedrich_amd import _capi as C
+
+    X, Xq = np.zeros((10, 3), order="F"), np.zeros((4, 3), order="F")
+    off, e, w = np.array([0, 4, 10]), np.zeros((4, 2), np.int32, order="F"), np.zeros((4, 2), order="F")
+    for spec in (["squared_exp", 0.5, 2.0], ("sum", ["squared_exp", 0.5, 2.0], ("linear", 0.1)), C.kprog(("squared_exp", 0.5, 2.0))):
+        ctx.experts_predict(spec, X, np.zeros(10), off, Xq, e, w)
+        ctx.experts_backward(spec, X, off, Xq, e, w, w, np.zeros(4))
+    assert [n for n, _ in ctx.lib.calls] == ["fr_experts_predict", "fr_experts_backward"] * 3
