@@ -527,6 +527,8 @@ class Context:
         """(K + noise^2 I) V for an Exponential kernel on ordered inputs t (fr_markov_product): gram + gemm in O(n)"""
         p = C.kprog(kernel)
         v = _Mat(V)
+        if _is_torch(t) and (_code(t) != C.FR_F64 or not t.is_contiguous()):
+            raise ValueError("t: has to be contiguous and float64")
         tp, nt, keep = _vecptr(t)
         if nt != v.rows:
             raise FriedrichError(C.FR_SHAPE, "inputs and rows differ")

@@ -131,3 +131,14 @@ def test_kernels_given_as_lists(ctx):
         ctx.experts_predict(spec, X, np.zeros(10), off, Xq, e, w)
         ctx.experts_backward(spec, X, off, Xq, e, w, w, np.zeros(4))
     assert [n for n, _ in ctx.lib.calls] == ["fr_experts_predict", "fr_experts_backward"] * 3
+
+
+def test_inputs_of_a_markov_product(ctx):
+    """inputs of another type or with gaps would be read beyond their end"""
+    V = columns(10, 2)
+    for t in (there(10, dtype=torch.float32), there(20)[::2], there(10, dtype=torch.float16)):
+        with pytest.raises(ValueError, match="t: "):
+            ctx.markov_product(("exponential", 1.0, 1.0), t, V)
+    assert not ctx.lib.calls
+    for t in (there(10), there(10, 1), np.arange(10), np.arange(20.0)[::2]):
+        ctx.markov_product(("exponential", 1.0, 1.0), t, V)
