@@ -200,28 +200,40 @@ __device__ __forceinline__ unsigned claim_tile(const RecArgs& a, unsigned* slot)
 //
 // A is a product of gates that may leave the type's range where no state does: gates beyond 1 over many rows.  What such an infinite A is
 // multiplied by may be 0 row by row -- a state of 0, or an A of 0 in front of it (a gate of 0 forgets) -- and then stays 0: the rows' own
-// values are in H, and inf * 0 would be a NaN of none of them.
-template <typename S>
+// values are in H, and inf * 0 would be a NaN of none of them.  Where every lane joins maps it does so without these looks (CHECKED = false) and
+// once more with them if a NaN came out: they took 4 % of 4194307 x 4 f64 rows.
+template <bool CHECKED, typename S>
 __device__ __forceinline__ S apply(S A, S state, S H)
 {
-    return state == S(0) ? H : A * state + H;
+    return CHECKED && state == S(0) ? H : A * state + H;
 }
-template <typename S>
+template <bool CHECKED, typename S>
 __device__ __forceinline__ S chain(S first, S then)
 {
-    return first == S(0) ? first : first * then;
+    return CHECKED && first == S(0) ? first : first * then;
 }
 template <typename S>
 struct Map {
     S A, H;
     bool cut;
-    __device__ __forceinline__ S of(S state) const { return cut ? H : apply(A, state, H); }
+    __device__ __forceinline__ bool nan() const { return A != A || H != H; }
+    template <bool CHECKED>
+    __device__ __forceinline__ S of(S state) const
+    {
+        return cut ? H : apply<CHECKED>(A, state, H);
+    }
 };
 // first p, then q
-template <typename S>
+template <bool CHECKED, typename S>
 __device__ __forceinline__ Map<S> join(const Map<S>& p, const Map<S>& q)
 {
-    return {chain(p.A, q.A), q.of(p.H), p.cut || q.cut};
+    return {chain<CHECKED>(p.A, q.A), q.template of<CHECKED>(p.H), p.cut || q.cut};
+}
+// joins without the looks for zeros, and once more with them where the first way says that a NaN came out
+template <class F>
+__device__ __forceinline__ void joined(F&& work)
+{
+    if (__any(work(std::false_type()))) work(std::true_type());
 }
 template <typename S>
 __device__ __forceinline__ Map<S> shift_up(const Map<S>& m, int step)
@@ -477,10 +489,15 @@ __global__ __launch_bounds__(512) void rec_rows_kernel(const RecArgs a)
         for (int v = 0; v < V; ++v) {
             before[v] = {S(1), S(0), false};
             if constexpr (!UNIFORM) {
-                for (int d = across; d < 64; d *= 2) {
-                    const Map<S> p = shift_up(m[v], d);
-                    if (lane >= d) m[v] = join(p, m[v]);
-                }
+                const Map<S> own = m[v];
+                joined([&](auto checked) {
+                    m[v] = own;
+                    for (int d = across; d < 64; d *= 2) {
+                        const Map<S> p = shift_up(m[v], d);
+                        if (lane >= d) m[v] = join<decltype(checked)::value>(p, m[v]);
+                    }
+                    return m[v].nan();
+                });
                 const Map<S> p = shift_up(m[v], across);
                 if (group > 0) before[v] = p;
             }
@@ -496,8 +513,12 @@ __global__ __launch_bounds__(512) void rec_rows_kernel(const RecArgs a)
                 const int64_t ch = ((int64_t)(item % (unsigned)a.blocks) * across + lane) * V + v;
                 S st = S(0);
                 if (a.tiles > 1 && ch < a.d) {
-                    Map<S> all = {mapA[0][v][lane], mapH[0][v][lane], mapC[0][v][lane] != 0};
-                    for (int k = 1; k < waves; ++k) all = join(all, Map<S>{mapA[k][v][lane], mapH[k][v][lane], mapC[k][v][lane] != 0});
+                    Map<S> all;
+                    joined([&](auto checked) {
+                        all = {mapA[0][v][lane], mapH[0][v][lane], mapC[0][v][lane] != 0};
+                        for (int k = 1; k < waves; ++k) all = join<decltype(checked)::value>(all, Map<S>{mapA[k][v][lane], mapH[k][v][lane], mapC[k][v][lane] != 0});
+                        return all.nan();
+                    });
                     unsigned long long* words = (unsigned long long*)a.maps;
                     unsigned long long* states = (unsigned long long*)a.carry;
                     publish(words + (pos * a.d + ch) * kMapWords<S>, all);
@@ -519,35 +540,56 @@ __global__ __launch_bounds__(512) void rec_rows_kernel(const RecArgs a)
                             if (ok || lost) break;
                             __builtin_amdgcn_s_sleep(1);
                         }
+                        const Map<S> so_far = sum;
+                        joined([&](auto checked) {
+                            sum = so_far;
 #pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            if (k0 + k < ahead) sum = join(sum, seen[k]);
+                            for (int k = 0; k < 8; ++k)
+                                if (k0 + k < ahead) sum = join<decltype(checked)::value>(sum, seen[k]);
+                            return sum.nan();
+                        });
                     }
-                    if (lost) {
-                        sum = {S(1), S(NAN), true};
-                        raise_lost(a);
-                    }
+                    if (lost) sum = {S(1), S(NAN), true};
+                    Map<S> onward;
+                    joined([&](auto checked) {
+                        onward = join<decltype(checked)::value>(sum, all);
+                        return onward.nan();
+                    });
                     for (int poll = 0; block > 0; ++poll) {
                         if (get_state(states + (block - 1) * a.d + ch, st)) break;
                         if (poll == a.polls) {
                             st = S(NAN);
-                            raise_lost(a);
+                            lost = true;
                             break;
                         }
                     }
-                    if (ahead == kRowsWindow - 1) put_state(states + block * a.d + ch, join(sum, all).of(st));
-                    st = sum.of(st);
+                    S through = S(0), front_of = S(0);
+                    joined([&](auto checked) {
+                        constexpr bool CHECKED = decltype(checked)::value;
+                        through = onward.template of<CHECKED>(st);
+                        front_of = sum.template of<CHECKED>(st);
+                        return through != through || front_of != front_of;
+                    });
+                    if (ahead == kRowsWindow - 1) put_state(states + block * a.d + ch, through);
+                    st = front_of;
+                    if (lost) raise_lost(a);
                 }
                 front[v][lane] = st;
             }
         }
         __syncthreads();
+        joined([&](auto checked) {
+            constexpr bool CHECKED = decltype(checked)::value;
+            bool nan = false;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            S st = front[v][cl];
-            for (int k = 0; k < wave; ++k) st = Map<S>{mapA[k][v][cl], mapH[k][v][cl], mapC[k][v][cl] != 0}.of(st);
-            state[v] = before[v].of(st);
-        }
+            for (int v = 0; v < V; ++v) {
+                S st = front[v][cl];
+                for (int k = 0; k < wave; ++k) st = Map<S>{mapA[k][v][cl], mapH[k][v][cl], mapC[k][v][cl] != 0}.template of<CHECKED>(st);
+                state[v] = before[v].template of<CHECKED>(st);
+                nan |= state[v] != state[v];
+            }
+            return nan;
+        });
     } else {
 #pragma unroll
         for (int v = 0; v < V; ++v) state[v] = S(0);
@@ -730,11 +772,12 @@ __global__ __launch_bounds__(512) void rec_columns_kernel(const RecArgs a)
 
     auto load = [&](const T* p) {  // E elements of a column from row0; rows that are not there: 0
         Run<T, E> r;
+        p += row0;  // (outside the branches: an address worked out in one took registers that a load of the other was still to fill, and waited)
         if (there && row0 + E <= a.n)
-            r = load_run<T, E>(p + row0);
+            r = load_run<T, E>(p);
         else
 #pragma unroll
-            for (int i = 0; i < E; ++i) r.v[i] = there && row0 + i < a.n ? p[row0 + i] : narrow<T>(S(0));
+            for (int i = 0; i < E; ++i) r.v[i] = there && row0 + i < a.n ? p[i] : narrow<T>(S(0));
         return r;
     };
 
@@ -806,31 +849,39 @@ __global__ __launch_bounds__(512) void rec_columns_kernel(const RecArgs a)
     };
 
     // the map of the lane's rows (the channels share its factor), of the rows of the lanes before it, and of the wave
-    S A = S(1), H[CG];
-    bool cut = enters != 0;
+    S A, H[CG];
+    bool cut;
+    joined([&](auto checked) {
+        constexpr bool CHECKED = decltype(checked)::value;
+        A = S(1), cut = enters != 0;
 #pragma unroll
-    for (int j = 0; j < CG; ++j) H[j] = S(0);
+        for (int j = 0; j < CG; ++j) H[j] = S(0);
 #pragma unroll
-    for (int i = 0; i < E; ++i)
-        if (valid >> i & 1) {
+        for (int i = 0; i < E; ++i)
+            if (valid >> i & 1) {
 #pragma unroll
-            for (int j = 0; j < CG; ++j) step(i, u[j][i], H[j], H[j]);
-            A *= ga[i];
+                for (int j = 0; j < CG; ++j) step(i, u[j][i], H[j], H[j]);
+                A *= ga[i];
+            }
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const S pa = __shfl_up(A, d);
+            const bool pc = __shfl_up((int)cut, d);
+#pragma unroll
+            for (int j = 0; j < CG; ++j) {
+                const S ph = __shfl_up(H[j], d);
+                if (lane >= d && !cut) H[j] = apply<CHECKED>(A, ph, H[j]);
+            }
+            if (lane >= d) {
+                A = chain<CHECKED>(pa, A);
+                cut = cut || pc;
+            }
         }
+        bool nan = A != A;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const S pa = __shfl_up(A, d);
-        const bool pc = __shfl_up((int)cut, d);
-#pragma unroll
-        for (int j = 0; j < CG; ++j) {
-            const S ph = __shfl_up(H[j], d);
-            if (lane >= d && !cut) H[j] = apply(A, ph, H[j]);
-        }
-        if (lane >= d) {
-            A = chain(pa, A);
-            cut = cut || pc;
-        }
-    }
+        for (int j = 0; j < CG; ++j) nan |= H[j] != H[j];
+        return nan;
+    });
     if (lane == 63) {
         mapA[wave] = A;
         mapC[wave] = cut;
@@ -850,8 +901,9 @@ __global__ __launch_bounds__(512) void rec_columns_kernel(const RecArgs a)
     for (int j = wave; j < ng; j += waves) {
         S st = S(0);
         if (a.tiles > 1) {
+            // (one lane's joins here and below: the looks for zeros cost less than a second way)
             Map<S> all = {mapA[0], mapH[j][0], mapC[0] != 0};
-            for (int k = 1; k < waves; ++k) all = join(all, Map<S>{mapA[k], mapH[j][k], mapC[k] != 0});
+            for (int k = 1; k < waves; ++k) all = join<true>(all, Map<S>{mapA[k], mapH[j][k], mapC[k] != 0});
             // (a channel's words lie side by side: a wave reads the window's in a few lines)
             unsigned long long* words = (unsigned long long*)a.maps + (c0 + j) * a.tiles * kMapWords<S>;
             unsigned long long* states = (unsigned long long*)a.carry + (c0 + j) * (a.tiles / kColumnsWindow + 1);
@@ -868,40 +920,44 @@ __global__ __launch_bounds__(512) void rec_columns_kernel(const RecArgs a)
                 __builtin_amdgcn_s_sleep(2);
             }
             if (lane >= ahead) m = {S(1), S(0), false};
-            if (lost) {
-                m = {S(1), S(NAN), true};
-                if (lane == 0) raise_lost(a);
-            }
+            if (lost) m = {S(1), S(NAN), true};
 #pragma unroll
             for (int d = 1; d < 64; d *= 2) {
                 const Map<S> p = shift_up(m, d);
-                if (lane >= d) m = join(p, m);
+                if (lane >= d) m = join<true>(p, m);
             }
             m = {__shfl(m.A, 63), __shfl(m.H, 63), (bool)__shfl((int)m.cut, 63)};
-            const Map<S> through = join(m, all);
+            const Map<S> through = join<true>(m, all);
             for (int poll = 0; window > 0; ++poll) {
                 if (get_state(states + window - 1, st)) break;
                 if (poll == a.polls) {
                     st = S(NAN);
-                    if (lane == 0) raise_lost(a);
+                    lost = true;
                     break;
                 }
                 __builtin_amdgcn_s_sleep(1);
             }
-            if (ahead == kColumnsWindow - 1 && lane == 0) put_state(states + window, through.of(st));
-            st = m.of(st);
+            if (ahead == kColumnsWindow - 1 && lane == 0) put_state(states + window, through.template of<true>(st));
+            st = m.template of<true>(st);
+            if (lost && lane == 0) raise_lost(a);
         }
         if (lane == 0) front[j] = st;
     }
     __syncthreads();
     S state[CG];
+    joined([&](auto checked) {
+        constexpr bool CHECKED = decltype(checked)::value;
+        bool nan = false;
 #pragma unroll
-    for (int j = 0; j < CG; ++j) {
-        if (j >= ng) continue;
-        S st = front[j];
-        for (int k = 0; k < wave; ++k) st = Map<S>{mapA[k], mapH[j][k], mapC[k] != 0}.of(st);
-        state[j] = cut ? H[j] : apply(A, st, H[j]);
-    }
+        for (int j = 0; j < CG; ++j) {
+            if (j >= ng) continue;
+            S st = front[j];
+            for (int k = 0; k < wave; ++k) st = Map<S>{mapA[k], mapH[j][k], mapC[k] != 0}.template of<CHECKED>(st);
+            state[j] = cut ? H[j] : apply<CHECKED>(A, st, H[j]);
+            nan |= state[j] != state[j];
+        }
+        return nan;
+    });
 
     if constexpr (!BACKWARD) {
         S* last = (S*)a.last;
