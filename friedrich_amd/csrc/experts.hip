@@ -38,8 +38,9 @@ __device__ __forceinline__ int64_t block_index(int64_t row, int64_t f, int64_t d
 
 // A workgroup per expert: every wave counts, among its share of the queries, the slots that name this expert and those that name an earlier
 // one, which is where the expert's list begins; a second walk puts each slot in its place, and the workgroup packs its list's query
-// points.  No atomics: a list's order is that of (share, j, q) on every run.  Every workgroup reads all slots (16384 slots: 64 KB, from
-// L2), which costs less than a launch to sort them first.  Bound by
+// points.  No atomics: a list's order is that of (share, j, q) on every run.  Every workgroup reads all slots twice (16384 slots: 64 KB, from
+// L2), which costs less than a launch to sort them first while experts times slots are few: 64 x 16384 are 0.1 GB, 1024 x 2^20 would be 8.6 GB
+// and take longer than the products of experts of 64 points.  Bound by
 // latency, the two walks and the packing behind them: 6.5 us for 6 slots of 16 experts, 14 us for 16384 slots of 64 experts and 65536 points of 16
 // features (8 MB read and written).  The list stays in LDS where it fits: written to memory and read again it took 1 us more.
 // (loads under a condition are waited for one by one: out of range they read the last place instead)
@@ -320,8 +321,9 @@ __device__ __forceinline__ int expert_of(const BlockArgs& a, const int64_t* item
 
 // A lane for each row of the columns' side, the sum over the blocks: an item is a wave of 64 lanes times a piece of blocks.  FOURS > 0: the
 // lanes' features stay in registers; 0: there are more than 16, and they are read again for every block.  Bound by issue of f64
-// instructions: 16777216 pairs of 16 features (squared exponential, 64 experts of 500 to 1500 points) take
-// 51 us, where 54 instructions a pair would take 23; 7500000 in the backward pass 27 us.  40 items a CU, on no more workgroups than the chip
+// instructions, which take three fifths of the SIMDs' time: 16777216 pairs of 16 features (squared exponential, 64 experts of 500 to 1500
+// points) take 51 us, where 54 instructions a pair would take 23; the rest are lanes of partial tiles, waits for scalar loads and uneven
+// ends; 7500000 in the backward pass 27 us.  40 items a CU, on no more workgroups than the chip
 // holds, even skewed experts out: whole calls with 20 items on 8 workgroups took 74 and 41 us, with 40 on 5 70 and 39, with 80 on 5 75 and 48.
 template <int LEAF, int FOURS>
 __global__ __launch_bounds__(256) void experts_lanes_kernel(const BlockArgs a)

@@ -62,7 +62,7 @@ __device__ __forceinline__ int64_t seq_of(const RecArgs& a, int64_t r)
     return lo;
 }
 
-// exp(g) and 1 - exp(g) from one polynomial: g = n ln 2 + r with |r| <= 0.3466 (two fused steps), q = exp(r) - 1 by its Taylor series
+// exp(g) and 1 - exp(g) from one polynomial: g = n ln 2 + r with |r| <= 0.3466 (ln 2 in two parts, after Cody and Waite, two fused steps), q = exp(r) - 1 by its Taylor series
 // (remainder 0.3466^14 / 14! = 4e-18 in f64, 0.3466^8 / 8! = 5e-9 in f32), exp(g) = 2^n (1 + q).  For n = 0, where 1 - exp(g) would cancel, it
 // is -q itself; elsewhere exp(g) is at most 0.71 or at least 1.41 and the difference is exact to a rounding or two.  Against exp, expm1 and
 // sqrt of the library (about 100 instructions in f64) this is about 45.
@@ -353,10 +353,13 @@ __device__ __forceinline__ void find_wave_edges(const RecArgs& a, int64_t lo, in
 // (64 channel lanes), so rows, their addresses and what begins and ends in them are the same for the whole wave and cost no vector
 // instruction; a stretch inside one sequence then runs without a branch.
 //
-// bf16, a gate for 128 channels, 37 sequences of 16413 rows x 2048 channels: backward 203 MB in 84 us, 2.4 TB/s (with vector
-// addresses and edges looked for in every row 113 and more).  The rest is the wait for the maps in front and the tail: a workgroup of 8 waves fills the
+// bf16, a gate for 128 channels, 37 sequences of 16413 rows x 2048 channels: backward 203 MB in 96 us on inputs that change from call to
+// call, 2.1 TB/s; 84 on the same ones (with vector addresses and edges looked for in every row 113 and more).  Vector instructions issue in
+// 22 % of that.  The rest is the wait for the maps in front and the tail: a workgroup of 8 waves fills the
 // registers of its CU, so loading, waiting and storing take turns.  3, 4 and 6 waves, windows of 8 and 32 tiles and 128 registers a lane were no
-// faster.  24 sequences of one row: the launch.
+// faster.  Rows of fewer than 64 channels, or of channels that share a gate in pairs, are further off: a lane holds one channel there, 2 bytes
+// of a 16-bit type (2^23 elements of f16: 36 to 50 MB in 49 to 70 us).  24 sequences of one row: 11 us, where a small launch takes 4; offsets,
+// rows, maps and given states are trips to memory one after the other, on four workgroups.
 
 template <typename T, int FORM, int V, bool SHARED, bool BACKWARD, bool UNIFORM, bool FEW>
 __global__ __launch_bounds__(512) void rec_rows_kernel(const RecArgs a)
@@ -741,8 +744,10 @@ __global__ __launch_bounds__(512) void rec_rows_kernel(const RecArgs a)
 // A lane holds E neighbouring rows of up to CG channels that share their gate, a workgroup 64 E rows a wave.  The gate is read, and its
 // exponential worked out, once for those channels.
 //
-// f64, three channels on one gate, 1000003 x 3 backward: 112 MB in 32 us, 3.5 TB/s; four on one, 4194307 x 4 forward: 302 MB in 104 us, 2.9 TB/s.
-// Bound as the rows are, by tiles that load, wait and store in turn (with blocks of 256 tiles and a map's words apart for each channel 149; 16 waves of 4
+// f64, three channels on one gate, 1000003 x 3 backward: 112 MB in 39 us on inputs that change from call to call, 2.9 TB/s (32 on the same ones,
+// which the last-level cache holds); four on one, 4194307 x 4 forward: 302 MB in 111 us, 2.7 TB/s.
+// Bound as the rows are, by tiles that load, wait and store in turn; 16-bit types load 16 bytes a lane and are further off (2^23 elements of
+// f16, 8 columns: 50 MB in 49 us; 1000 columns of 300 sequences 66, where every lane near an edge searches the offsets).  (With blocks of 256 tiles and a map's words apart for each channel 149; 16 waves of 4
 // rows a lane 99, but 44 instead of 40 where there is one channel).
 
 template <typename T, int FORM, int CG, bool BACKWARD>

@@ -230,7 +230,9 @@ __global__ __launch_bounds__(256) void route_general_kernel(const RouteArgs a)
 // the larger double), so that exchanging two entries is one maximum and one minimum.  Keys that are logits of 32 bits or less are exact.  Others
 // are 2^-19 (1 + |key|) from the 64-bit value or nearer: a row in which two keys that matter lie closer together, or where a key is not finite,
 // is left to a second launch, which gives it a wave and orders it in 64 bits.  (64-bit keys throughout took 2430 instructions for four rows of 256 experts, 770 of them
-// in the sigmoids, and 157 us for 65536 rows; this takes about 1300, and 84 us with the second launch and the counts: bound by issue.)
+// in the sigmoids, and 157 us for 65536 rows; this takes about 1200, and 84 us with the second launch and the counts.  They issue in just
+// under half of the first launch's 68 us: 196 registers leave two waves a SIMD to cover each other's waits, and 226 of the code's 1628 vector
+// instructions move spilled scalars.)  A bias that closes an expert makes every row one to be done again: 418 us.
 
 __device__ __forceinline__ double at_bits(unsigned long long b) { return __longlong_as_double((long long)b); }
 __device__ __forceinline__ unsigned long long bits_of(double v) { return (unsigned long long)__double_as_longlong(v); }
@@ -542,9 +544,10 @@ __global__ __launch_bounds__(256) void route_again_kernel(const RouteArgs a)
     for (int i = threadIdx.x >> 6; i < count; i += 4) route_row<T, J, SIGMOID>(a, a.again[blockIdx.x * a.room + i], a.partial ? a.partial + (int64_t)blockIdx.x * a.experts : nullptr);
 }
 
-// Each lane writes its experts' gradients as if none of them had been chosen and then, over it, those of the experts that were.  Bound by issue of
-// the f64 exponentials: 32768 x 128 bf16, k = 4, 15.8 us alone and 14 in a row of calls, 1.3 TB/s of the 17.8 MB that it reads and writes; with the slots'
-// number not known when compiled, 1.5 us more.  33 rows of 16: 4 us.
+// Each lane writes its experts' gradients as if none of them had been chosen and then, over it, those of the experts that were.  32768 x 128
+// bf16, k = 4: 15 to 16 us alone and 14 in a row of calls, 1.3 TB/s of the 17.8 MB that it reads and writes; vector instructions issue in
+// two thirds of that, and of the code's 1940 a quarter are moves between registers (the two-address multiply-adds of the series) and a fifth the
+// exponentials of the row.  With the slots' number not known when compiled, 1.5 us more.  33 rows of 16: 4 us.
 template <typename T, int C, int K, bool SIGMOID>
 __global__ __launch_bounds__(256) void route_backward_kernel(const RouteArgs a)
 {

@@ -424,7 +424,8 @@ int fr_route_backward(fr_ctx* ctx, int dtype, int layout, int score, int64_t n, 
  * fr_route gives, k <= 64; slots outside [0, n_experts) have a mean of 0.
  *   out_slots[q, j] = sum_i k(x_q, x_i) alpha_i over the points of experts[q, j]    (m x k; may be NULL)
  *   out_mean[q]     = prior_q[q] + sum_j weights[q, j] out_slots[q, j]             (prior_q NULL: 0)
- * One expert with weight 1 is fr_predict_mean with its cached alpha.  The sums' order is fixed by the arguments. */
+ * One expert with weight 1 is fr_predict_mean with its cached alpha.  The sums' order is fixed by the arguments.  Collecting the experts'
+ * slots reads 8 n_experts m k bytes, forward and backward (from cache): 0.07 GB for 64 experts and 2^17 slots, 8.6 GB for 1024 and 2^20. */
 int fr_experts_predict(fr_ctx* ctx, const fr_kprog* kernel, const double* X, int64_t n, int64_t ldx, int64_t d, const double* alpha,
                        const void* offsets, int64_t n_experts, const double* Xq, int64_t m, int64_t ldq, const void* experts, int64_t lde,
                        const double* weights, int64_t ldw, int64_t k, const double* prior_q, double* out_mean, double* out_slots, int64_t lds);
