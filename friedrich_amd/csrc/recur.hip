@@ -87,6 +87,8 @@ int fr_recurrence(fr_ctx* ctx, int dtype, int layout, int form, int64_t n, int64
     return op_entry(ctx, [&]() -> int {
         FR_TRY(rec_check(ctx, dtype, layout, form, n, d, gate_cols, offsets, nseq));
         if (d == 0 || nseq == 0) return FR_OK;
+        // (a tile reads the states that its sequences enter with twice; another may have written those that they leave with in between)
+        if (h_last && h_last == h0) return set_err(ctx, FR_INVALID_ARGUMENT, "h_last: the same memory as h0");
         const int64_t e = dtype_size(dtype), w = wide_size(dtype);
         Operand o(ctx), og(ctx), ox(ctx), oh0(ctx), oh(ctx), ol(ctx);
         FR_TRY(rec_offsets(ctx, o, offsets, nseq, n));
@@ -117,6 +119,7 @@ int fr_recurrence_backward(fr_ctx* ctx, int dtype, int layout, int form, int64_t
     return op_entry(ctx, [&]() -> int {
         FR_TRY(rec_check(ctx, dtype, layout, form, n, d, gate_cols, offsets, nseq));
         if (d == 0 || nseq == 0 || !(dgate || dx || dh0)) return FR_OK;
+        if (dh0 && dh0 == dh_last) return set_err(ctx, FR_INVALID_ARGUMENT, "dh0: the same memory as dh_last");  // (as h_last and h0)
         const int64_t e = dtype_size(dtype), w = wide_size(dtype);
         Operand o(ctx), og(ctx), ox(ctx), oh0(ctx), oh(ctx), odh(ctx), odl(ctx), odg(ctx), odx(ctx), odh0(ctx);
         FR_TRY(rec_offsets(ctx, o, offsets, nseq, n));
@@ -165,6 +168,7 @@ int fr_markov_product(fr_ctx* ctx, const fr_kprog* kernel, const double* t, int6
             for (int64_t i = 1; i < n; ++i)
                 if (!(t[i] >= t[i - 1])) return set_err(ctx, FR_INVALID_ARGUMENT, "t[%lld] lies before the input in front of it", (long long)i);
         if (n == 0 || m == 0) return FR_OK;
+        if (out == V) return set_err(ctx, FR_INVALID_ARGUMENT, "out: the same memory as V");  // (V is read again when out is joined)
         const double ls = kernel->ops[0].params[0], ampl = std::fabs(kernel->ops[0].params[1]);
         OpWorkspace ws(ctx);
         FR_TRY(ws.get(sizeof(double) * (size_t)(n + n * m)));

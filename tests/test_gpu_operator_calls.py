@@ -171,3 +171,28 @@ def test_a_context_on_its_own_stream():
         assert torch.equal(e + 0, want_r[0]) and torch.equal(w + 0, want_r[1])
     c.close()
     ref.close()
+
+
+@pytest.mark.parametrize("layout", ["row", "col"])
+def test_states_are_not_carried_in_place(tctx, layout):  # noqa: F811
+    """the states behind the sequences over those in front of them, and a product over its factor: memory that is read again after it
+    has been written, so refused"""
+    import torch
+    from friedrich_amd import _capi as C
+    from friedrich_amd.device import FriedrichError
+
+    rng = np.random.default_rng(65)
+    gate, x, h0, _ = problem(rng, 300, 5, 5, 1, "log", "f32", layout)
+    V = put(rng.standard_normal((50, 2)), "col", torch.float64)
+    t = torch.arange(50, dtype=torch.float64, device="cuda")
+    refused = [lambda: tctx.recurrence(gate, x, h0=h0, last=h0), lambda: tctx.recurrence_backward(gate, x, x, x.clone(), dlast=h0, dh0=h0),
+               lambda: tctx.markov_product(("exponential", 1.0, 1.0), t, V, out=V)]
+    host_state = np.zeros((1, 5), np.float32, order="F")
+    refused.append(lambda: tctx.recurrence(np.zeros((9, 5), np.float32, order="F"), np.ones((9, 5), np.float32, order="F"), h0=host_state, last=host_state))
+    for call in refused:
+        with pytest.raises(FriedrichError) as e:
+            call()
+        assert e.value.status == C.FR_INVALID_ARGUMENT
+    before = h0.clone()
+    _, last = tctx.recurrence(gate, x, h0=h0)
+    assert torch.equal(h0, before) and not torch.equal(last, h0)
